@@ -153,9 +153,9 @@ def _quantize_rows(x):
     x = x.float()
     top = x.abs().amax(dim=1)
     live = top >= _TINY
-    inv = torch.where(live, 127.0 / top, 0.0)
-    q = torch.round(x * inv[:, None]).to(torch.int8)
-    return q, torch.where(live, top / 127.0, 0.0)
+    full = torch.full_like(top, 127.0)            # tensor by tensor: torch turns a scalar divisor into a product
+    q = torch.round(x * torch.where(live, full / top, 0.0)[:, None]).to(torch.int8)
+    return q, torch.where(live, top / full, 0.0)
 
 
 def _product(q, s, wq, ws):
