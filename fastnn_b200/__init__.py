@@ -7,9 +7,10 @@ CPU fallback: importing works anywhere, computing needs the library and a B200.
 """
 from ._lib import LibraryMissing, lib, library_path  # noqa: F401
 from .cuda_backend import (  # noqa: F401
-    ACT_GELU, ACT_NONE, ACT_RELU, NN, NT, TN, CudaError, attention_forward, conv2d_backward, conv2d_forward, cuda_init, cuda_matmul, cuda_matmul_batched,
+    ACT_GELU, ACT_NONE, ACT_RELU, ACT_SILU, NN, NT, TN, CudaError, attention_forward, conv2d_backward, conv2d_forward, cuda_init, cuda_matmul, cuda_matmul_batched,
     cuda_matmul_batched_nt, cuda_matmul_batched_tn, cuda_matmul_nt, cuda_matmul_tn, device_status,
-    current_stream_ptr, gemm_ex, gemm_gather_ex, gemm_gather_mc_ex, gemm_splitk_static, selftest_bounded_wait, gru_pack_weights, last_path, reduce_partials, launch_count, linear_backward_input, linear_forward, matmul, matmul_nt, matmul_tn, plan_query, rnn_gates_forward, set_policy,
+    current_stream_ptr, gemm_ex, gemm_gather_ex, gemm_gather_mc_ex, gemm_splitk_static, selftest_bounded_wait, gated_ffn_backward, gated_ffn_forward, gru_pack_weights, int8_gated_forward, int8_linear_forward,
+    last_path, reduce_partials, launch_count, linear_backward_input, linear_forward, matmul, matmul_nt, matmul_tn, plan_query, quantize_rows, rnn_gates_forward, set_policy,
     synchronize,
 )
 

@@ -60,6 +60,14 @@ SIGNATURES = {
                                         _f, _vp, _i, ctypes.POINTER(_vp), _i, _vp]),
     "fastnn_b200_gemm_gather_mc_ex": (_i, [_i, _vp, _vp, _vp, _i, _i, _i, _i, _ll, _ll, _ll, _ll, _ll, _ll,
                                            _f, _vp, _i, _vp, _vp]),
+    "fastnn_b200_gated_ffn_workspace": (ctypes.c_size_t, [_i] * 6),
+    "fastnn_b200_gated_ffn_forward": (_i, [_i, _vp, _ll] + [_vp] * 6 + [_i] * 4 + [_vp, ctypes.c_size_t, _vp]),
+    "fastnn_b200_gated_ffn_backward": (_i, [_i, _vp, _ll, _vp, _ll] + [_vp] * 9 + [_i] * 4 +
+                                       [_vp, ctypes.c_size_t, _vp]),
+    "fastnn_b200_quantize_rows": (_i, [_i, _vp, _ll, _vp, _vp, _i, _i, _vp]),
+    "fastnn_b200_int8_workspace": (ctypes.c_size_t, [_i] * 5),
+    "fastnn_b200_int8_linear_forward": (_i, [_vp] * 6 + [_i] * 5 + [_vp, ctypes.c_size_t, _vp]),
+    "fastnn_b200_int8_gated_forward": (_i, [_vp] * 7 + [_i] * 5 + [_vp, ctypes.c_size_t, _vp]),
     "fastnn_b200_selftest_bounded_wait": (_i, [ctypes.c_uint, ctypes.POINTER(ctypes.c_uint)]),
     "fastnn_b200_reduce_partials": (_i, [_vp, _vp, _i, _i, _i, _ll, _f, _f, _vp, _i, _vp]),
     "fastnn_b200_set_policy": (_i, [_i, _i, _i]),

@@ -21,6 +21,8 @@
 #include "conv_tcgen05.cuh"
 #include "conv_wgrad_tcgen05.cuh"
 #include "conv_wgrad_slab_tcgen05.cuh"
+#include "narrow_gemm_tcgen05.cuh"
+#include "quantize_rows.cuh"
 
 namespace {
 
@@ -962,6 +964,8 @@ int resolve_encoder() {
   return 0;
 }
 
+int narrow_init();                  // narrow_host.cuh
+
 }  // namespace
 
 // ============================================================ drop-in symbols ===
@@ -1001,6 +1005,7 @@ extern "C" int fastnn_cuda_init(int device_id) {
                                    static_cast<int>(kMaxDynSmem)));
   FNN_CUDA_OK(cudaFuncSetAttribute(fnn::conv2d_wgrad_tf32_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                    static_cast<int>(kMaxDynSmem)));
+  if (narrow_init() != 0) return -1;
   st.num_sms = prop.multiProcessorCount;
   FNN_CUDA_OK(cudaFuncSetAttribute(fnn::gemm_tf32_clusterk_kernel,
                                    cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -2307,3 +2312,6 @@ extern "C" int fastnn_b200_gemm_splitk_static(int layout, const float* a, const 
   t_last = LastCall{2, block_n, split_k, grid};
   return 0;
 }
+
+// ================================ gated feed-forward block, 8-bit products ===
+#include "narrow_host.cuh"

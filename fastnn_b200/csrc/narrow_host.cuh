@@ -1,0 +1,652 @@
+// Host side of the gated feed-forward block and the 8-bit products: argument checks, the plan of each
+// launch, workspace layout, tensor maps.  Included once, by fastnn_api.cu.
+#pragma once
+
+namespace {
+
+constexpr int kDefaultClusters = 74;       // CTA pairs of a B200, for size queries without a device
+
+struct DType {
+  int code;            // FASTNN_B200_F32 / F16 / BF16, or -1: signed 8-bit
+  int bytes;
+  int kind;            // fnn::kKind*
+  CUtensorMapDataType map;
+};
+bool dtype_of(int code, DType* d) {
+  switch (code) {
+    case FASTNN_B200_F32: *d = DType{code, 4, fnn::kKindTf32, CU_TENSOR_MAP_DATA_TYPE_FLOAT32}; return true;
+    case FASTNN_B200_F16: *d = DType{code, 2, fnn::kKindF16, CU_TENSOR_MAP_DATA_TYPE_FLOAT16}; return true;
+    case FASTNN_B200_BF16: *d = DType{code, 2, fnn::kKindF16, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16}; return true;
+    default: return false;
+  }
+}
+const DType kInt8 = {-1, 1, fnn::kKindI8, CU_TENSOR_MAP_DATA_TYPE_UINT8};
+
+bool gate_act_ok(int act) {
+  return act == FASTNN_B200_ACT_NONE || act == FASTNN_B200_ACT_RELU || act == FASTNN_B200_ACT_GELU ||
+         act == FASTNN_B200_ACT_SILU;
+}
+
+// Tensor map of a row-major [d1, d0] matrix (x `d2` slices), 128-byte swizzle, zero outside.
+bool encode_narrow(CUtensorMap* map, const DType& t, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
+                   uint64_t pitch, uint64_t slice, uint32_t box0, uint32_t box1, bool atom32) {
+  const EncodeTiledFn encode = g_encode.load(std::memory_order_acquire);
+  if (encode == nullptr) return false;
+  MapKey key;
+  std::memset(&key, 0, sizeof(key));
+  key.base = base;
+  key.d[0] = d0; key.d[1] = d1; key.d[2] = d2;
+  key.s[0] = pitch; key.s[1] = slice;
+  key.box[0] = box0; key.box[1] = box1; key.box[2] = 1;
+  key.kind = 16u + 2u * static_cast<uint32_t>(t.map) + (atom32 ? 1u : 0u);
+  if (map_cache_get(key, map)) return true;
+  cuuint64_t dims[3] = {d0, d1, d2};
+  cuuint64_t strides[2] = {pitch, slice};
+  cuuint32_t box[3] = {box0, box1, 1};
+  cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = encode(map, t.map, 3, const_cast<void*>(base), dims, strides, box, estr,
+                            CU_TENSOR_MAP_INTERLEAVE_NONE,
+                            atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r == CUDA_SUCCESS) map_cache_put(key, *map);
+  return r == CUDA_SUCCESS;
+}
+
+// A row-major matrix as a call gives it; `ld` in elements.
+struct Mat {
+  const void* p;
+  long long ld;
+  int rows, cols;
+};
+inline long long round_up(long long v, long long to) { return (v + to - 1) / to * to; }
+inline bool rows_addressable(const void* p, long long ld, int bytes) {
+  return aligned16(p) && ((ld * bytes) & 15) == 0 && ld * bytes < (1ll << 40);
+}
+
+// Carves a call's workspace.  A dry one only adds up, which is how the size queries work: both
+// run the same code, so they cannot disagree.
+struct Carver {
+  uint8_t* base;
+  size_t bytes;
+  bool dry;
+  size_t used = 0;
+  void* take(size_t want) {
+    void* p = dry || base == nullptr ? nullptr : base + used;
+    used += (want + 255) & ~size_t(255);
+    return p;
+  }
+  // Whether the caller's buffer holds what was taken; asked once everything is, before the first launch.
+  bool fits() const {
+    if (used <= bytes && (used == 0 || (base != nullptr && aligned16(base)))) return true;
+    std::fprintf(stderr, "fastnn_b200: a workspace of %zu bytes on a 16-byte boundary is needed, %zu were given at %p\n",
+                 used, bytes, static_cast<void*>(base));
+    return false;
+  }
+};
+
+struct Packer {
+  fnn::PackParams p;
+  int blocks = 0;
+  Packer() { std::memset(&p, 0, sizeof(p)); }
+  // m as TMA can address it: itself, or a copy in the workspace with rows padded to 16 bytes
+  Mat fit(Carver& ws, const Mat& m, int bytes, bool pack) {
+    if (!pack) return m;
+    const long long pitch = round_up(1ll * m.cols * bytes, 16);
+    Mat out{ws.take(static_cast<size_t>(pitch) * m.rows), pitch / bytes, m.rows, m.cols};
+    if (!ws.dry) {
+      fnn::PackItem& it = p.it[p.count++];
+      it.src = static_cast<const uint8_t*>(m.p);
+      it.dst = static_cast<uint8_t*>(const_cast<void*>(out.p));
+      it.src_pitch = m.ld * bytes;
+      it.dst_pitch = pitch;
+      it.rows = m.rows;
+      it.row_bytes = m.cols * bytes;
+      it.first_block = blocks;
+      blocks += static_cast<int>((m.rows * (pitch >> 2) + fnn::kPackWords - 1) / fnn::kPackWords);
+    }
+    return out;
+  }
+  int launch(cudaStream_t s) {
+    if (blocks == 0) return 0;
+    fnn::pack_rows_kernel<<<blocks, 256, 0, s>>>(p);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    FNN_CUDA_OK(cudaGetLastError());
+    return 0;
+  }
+};
+
+// One product of a launch before its maps are made.
+struct NarrowTask {
+  Mat a[2], b[2];            // as stored; second pair optional (rows = 0), or b[1] = the up weight
+  bool a_mn = false, b_mn = false;
+  int m = 0, n = 0, k = 0, k2 = 0;
+  void* out[3] = {nullptr, nullptr, nullptr};
+  long long out_ld[3] = {0, 0, 0};
+  const void* gate = nullptr;
+  const void* up = nullptr;
+  long long aux_ld = 0;
+  // plan
+  int split = 1, kb_per_split = 0, num_kb1 = 0, num_kb = 0;
+  float* partials = nullptr;
+};
+
+struct NarrowPlan {
+  int block_n;
+};
+
+// Tile width and K split of a launch.  Cost in SM clocks of the busiest CTA pair: a 128-byte k-block of
+// a 256 x block_n tile takes the tensor cores 2 * block_n clocks and its loads (16 KiB of A and
+// block_n / 2 rows of B per CTA) 1 / 64 clock a byte; a unit costs about 2000 clocks beside its k-blocks
+// (pipeline fill, the drain of its accumulator at the end of a wave), and a K split the reduction's
+// bytes and launch.  Units go round robin over the pairs, so their sums are exact.
+NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool gated, bool may_split) {
+  int max_kb = 1;
+  for (int i = 0; i < count; ++i) {
+    t[i].num_kb1 = ceil_div(t[i].k, kblock);
+    t[i].num_kb = t[i].num_kb1 + (t[i].k2 > 0 ? ceil_div(t[i].k2, kblock) : 0);
+    if (t[i].num_kb > max_kb) max_kb = t[i].num_kb;
+  }
+  double best = 1e300;
+  int best_bn = 256, best_len = max_kb;
+  // a CTA's half of an MN-major B tile is whole 128-byte chunks of N
+  int min_bn = gated ? 128 : 64;
+  for (int i = 0; i < count; ++i)
+    if (t[i].b_mn && min_bn < 2 * kblock) min_bn = 2 * kblock;
+  for (int bn = min_bn; bn <= 256; bn *= 2) {
+    const double load = (fnn::kNarrowABytes + bn / 2 * 128) / 64.0;
+    const double per_kb = 2.0 * bn > load ? 2.0 * bn : load;
+    for (int parts = 1; parts <= (may_split ? 64 : 1); parts += parts < 8 ? 1 : (parts < 16 ? 2 : 8)) {
+      const int len = ceil_div(max_kb, parts);                  // k-blocks of a unit, at most
+      if (parts > 1 && len < 4) break;
+      double most = 0.0, reduce = 0.0;
+      int first = 0;
+      // units of problem i on pair c: those u in [first, first + units) with u % clusters == c
+      for (int c = 0; c < clusters; ++c) {
+        double sum = 0.0;
+        first = 0;
+        for (int i = 0; i < count; ++i) {
+          const int split = ceil_div(t[i].num_kb, len);
+          const int per = ceil_div(t[i].num_kb, split);
+          const int cols = gated ? bn / 2 : bn;
+          const long long units = 1ll * ceil_div(t[i].m, 256) * ceil_div(t[i].n, cols) * split;
+          const long long lo = (c - first % clusters + clusters) % clusters;
+          const long long mine = lo < units ? (units - lo + clusters - 1) / clusters : 0;
+          sum += mine * (per * per_kb + 2000.0);
+          first += static_cast<int>(units % clusters);
+        }
+        if (sum > most) most = sum;
+      }
+      for (int i = 0; i < count; ++i) {
+        const int split = ceil_div(t[i].num_kb, len);
+        if (split > 1) reduce += 8.0 * split * t[i].m * t[i].n / 3400.0 / 2.0;   // written and read, mostly in L2
+      }
+      if (reduce > 0.0) reduce += 5000.0;
+      const double cost = most + reduce;
+      if (cost < best) { best = cost; best_bn = bn; best_len = len; }
+    }
+  }
+  for (int i = 0; i < count; ++i) {
+    t[i].split = ceil_div(t[i].num_kb, best_len);
+    t[i].kb_per_split = ceil_div(t[i].num_kb, t[i].split);
+    t[i].split = ceil_div(t[i].num_kb, t[i].kb_per_split);
+  }
+  return NarrowPlan{best_bn};
+}
+
+inline long long partial_ld(const NarrowTask& t) { return round_up(t.n, 4); }
+void reserve_partials(Carver& ws, NarrowTask* t, int count) {
+  for (int i = 0; i < count; ++i)
+    if (t[i].split > 1)
+      t[i].partials = static_cast<float*>(ws.take(sizeof(float) * static_cast<size_t>(partial_ld(t[i])) * t[i].m * t[i].split));
+}
+
+typedef void (*NarrowKernel)(fnn::NarrowParams);
+// Every instantiation, for the shared-memory attribute and for dispatch: [dtype][epilogue]
+NarrowKernel pair_kernel(int kind, int epi, int out_code) {
+  using namespace fnn;
+  if (kind == kKindF16) {
+    const bool bf = out_code == FASTNN_B200_BF16;
+    if (epi == kEpiStore) return bf ? &narrow_pair_kernel<kKindF16, kEpiStore, __nv_bfloat16> : &narrow_pair_kernel<kKindF16, kEpiStore, __half>;
+    if (epi == kEpiGated) return bf ? &narrow_pair_kernel<kKindF16, kEpiGated, __nv_bfloat16> : &narrow_pair_kernel<kKindF16, kEpiGated, __half>;
+    if (epi == kEpiGatedGrad) return bf ? &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __nv_bfloat16> : &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __half>;
+  } else if (kind == kKindTf32) {
+    if (epi == kEpiStore) return &narrow_pair_kernel<kKindTf32, kEpiStore, float>;
+    if (epi == kEpiGated) return &narrow_pair_kernel<kKindTf32, kEpiGated, float>;
+    if (epi == kEpiGatedGrad) return &narrow_pair_kernel<kKindTf32, kEpiGatedGrad, float>;
+  } else {
+    if (epi == kEpiScaled)
+      return out_code == FASTNN_B200_F32 ? &narrow_pair_kernel<kKindI8, kEpiScaled, float>
+             : (out_code == FASTNN_B200_BF16 ? &narrow_pair_kernel<kKindI8, kEpiScaled, __nv_bfloat16>
+                                             : &narrow_pair_kernel<kKindI8, kEpiScaled, __half>);
+    if (epi == kEpiScaledGated)
+      return out_code == FASTNN_B200_F32 ? &narrow_pair_kernel<kKindI8, kEpiScaledGated, float>
+             : (out_code == FASTNN_B200_BF16 ? &narrow_pair_kernel<kKindI8, kEpiScaledGated, __nv_bfloat16>
+                                             : &narrow_pair_kernel<kKindI8, kEpiScaledGated, __half>);
+  }
+  return nullptr;
+}
+
+// Called once per device by fastnn_cuda_init.
+int narrow_init() {
+  const int codes[3] = {FASTNN_B200_F32, FASTNN_B200_F16, FASTNN_B200_BF16};
+  for (int kind = 0; kind <= 2; ++kind)
+    for (int epi = 0; epi <= 4; ++epi)
+      for (int c : codes) {
+        NarrowKernel k = pair_kernel(kind, epi, c);
+        if (k == nullptr) continue;
+        FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
+      }
+  return 0;
+}
+
+struct NarrowLaunch {
+  DType in;
+  int out_code;
+  int epi;
+  int act = 0;
+  const float* row_scale = nullptr;
+  const float* col_scale = nullptr;
+  const float* col_scale2 = nullptr;
+  const float* bias = nullptr;
+};
+
+int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int count, const NarrowPlan& plan,
+                cudaStream_t stream) {
+  using namespace fnn;
+  static thread_local NarrowParams p;
+  std::memset(&p, 0, sizeof(p));
+  const bool gated = l.epi == kEpiGated || l.epi == kEpiScaledGated;
+  const int kblock = 128 / l.in.bytes;
+  const uint32_t half_n = plan.block_n / 2;
+  DType out;
+  if (!dtype_of(l.out_code, &out)) return -1;
+  DType f32;
+  dtype_of(FASTNN_B200_F32, &f32);
+  bool ok = true;
+  long long units = 0;
+  for (int i = 0; i < count; ++i) {
+    const NarrowTask& q = t[i];
+    NarrowProblem& d = p.pr[i];
+    d.m = q.m; d.n = q.n;
+    d.tiles_m = ceil_div(q.m, 256);
+    d.tiles_n = ceil_div(q.n, gated ? static_cast<int>(half_n) : plan.block_n);
+    d.num_kb = q.num_kb; d.num_kb1 = q.num_kb1;
+    d.split_k = q.split; d.kb_per_split = q.kb_per_split;
+    d.first_unit = static_cast<int>(units);
+    units += 1ll * d.tiles_m * d.tiles_n * d.split_k;
+    if (units > 0x3fffffffll) return -1;
+    d.a_mn = q.a_mn ? 1 : 0; d.b_mn = q.b_mn ? 1 : 0;
+    const bool atom32 = l.in.kind == kKindTf32;
+    for (int j = 0; j < 2; ++j) {
+      if (q.a[j].rows > 0)
+        ok = ok && encode_narrow(&d.a[j], l.in, q.a[j].p, q.a[j].cols, q.a[j].rows, 1, q.a[j].ld * l.in.bytes,
+                                 q.a[j].ld * l.in.bytes * q.a[j].rows, kblock, q.a_mn ? kblock : 128, q.a_mn && atom32);
+      if (q.b[j].rows > 0)
+        ok = ok && encode_narrow(&d.b[j], l.in, q.b[j].p, q.b[j].cols, q.b[j].rows, 1, q.b[j].ld * l.in.bytes,
+                                 q.b[j].ld * l.in.bytes * q.b[j].rows, kblock, q.b_mn ? kblock : half_n, q.b_mn && atom32);
+    }
+    if (q.split > 1) {
+      const long long ld = partial_ld(q);
+      d.out_ptr[0] = q.partials;
+      d.tma_out[0] = 1;
+      ok = ok && encode_narrow(&d.out[0], f32, q.partials, q.n, q.m, q.split, ld * 4, ld * 4 * q.m, 32, 32, false);
+    } else {
+      for (int j = 0; j < 3; ++j) {
+        if (q.out[j] == nullptr) continue;
+        d.out_ptr[j] = q.out[j];
+        d.out_ld[j] = q.out_ld[j];
+        d.tma_out[j] = rows_addressable(q.out[j], q.out_ld[j], out.bytes) ? 1 : 0;
+        if (d.tma_out[j])
+          ok = ok && encode_narrow(&d.out[j], out, q.out[j], q.n, q.m, 1, q.out_ld[j] * out.bytes,
+                                   q.out_ld[j] * out.bytes * q.m, 128 / out.bytes, 32, false);
+      }
+    }
+    d.gate = q.gate; d.up = q.up; d.aux_ld = q.aux_ld;
+  }
+  if (!ok) return -1;
+  p.count = count;
+  p.total_units = static_cast<int>(units);
+  p.block_n = plan.block_n;
+  const size_t stage = kNarrowABytes + half_n * 128;
+  int stages = static_cast<int>((kMaxDynSmem - narrow_pair_smem_bytes(plan.block_n, 0)) / stage);
+  p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;
+  p.group_m = 8;
+  p.act = l.act;
+  p.is_bf16 = l.in.code == FASTNN_B200_BF16 ? 1 : 0;
+  p.row_scale = l.row_scale; p.col_scale = l.col_scale; p.col_scale2 = l.col_scale2; p.bias = l.bias;
+  p.status = st->status;
+  p.spin_budget = st->spin_budget;
+  const int clusters = p.total_units < st->max_clusters ? p.total_units : st->max_clusters;
+  NarrowKernel k = pair_kernel(l.in.kind, l.epi, l.out_code);
+  if (k == nullptr || clusters < 1) return -1;
+  k<<<2 * clusters, kNarrowThreads, narrow_pair_smem_bytes(p.block_n, p.num_stages), stream>>>(p);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  FNN_CUDA_OK(cudaGetLastError());
+  t_last = LastCall{12, plan.block_n, t[0].split, 2 * clusters};
+
+  NarrowReduceParams r;
+  std::memset(&r, 0, sizeof(r));
+  long long blocks = 0;
+  for (int i = 0; i < count; ++i) {
+    if (t[i].split <= 1) continue;
+    NarrowReduceItem& it = r.it[r.count++];
+    it.partials = t[i].partials;
+    it.out = t[i].out[0];
+    it.ld = partial_ld(t[i]);
+    it.slice = it.ld * t[i].m;
+    it.out_ld = t[i].out_ld[0];
+    it.rows = t[i].m; it.cols = t[i].n; it.slices = t[i].split;
+    it.first_block = static_cast<int>(blocks);
+    blocks += (1ll * t[i].m * ceil_div(t[i].n, kReduceCols) + 255) / 256;
+  }
+  if (blocks > 0) {
+    if (blocks > 0x7fffffffll) return -1;
+    const unsigned g = static_cast<unsigned>(blocks);
+    if (l.out_code == FASTNN_B200_F32) narrow_reduce_kernel<float><<<g, 256, 0, stream>>>(r);
+    else if (l.out_code == FASTNN_B200_BF16) narrow_reduce_kernel<__nv_bfloat16><<<g, 256, 0, stream>>>(r);
+    else narrow_reduce_kernel<__half><<<g, 256, 0, stream>>>(r);
+    g_launches.fetch_add(1, std::memory_order_relaxed);
+    FNN_CUDA_OK(cudaGetLastError());
+  }
+  return 0;
+}
+
+// ------------------------------------------------------------- gated feed-forward ---
+struct FfnArgs {
+  DType t;
+  int rows, d, f, act;
+  Mat x, wg, wu, wd, dy;
+  Mat gate, up;              // backward: saved; forward: outputs or null
+  void* y = nullptr;
+  void *dx = nullptr, *dwg = nullptr, *dwu = nullptr, *dwd = nullptr;
+};
+
+int clusters_of(const DeviceState* st) { return st != nullptr && st->max_clusters > 0 ? st->max_clusters : kDefaultClusters; }
+
+// Forward.  With ws.dry only the workspace is added up (pack_all: as if no operand were
+// addressable).
+int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cudaStream_t s) {
+  const int e = a.t.bytes;
+  const bool dry = ws.dry;
+  auto must_pack = [&](const Mat& m) { return dry ? pack_all || ((m.ld * e) & 15) != 0 : !rows_addressable(m.p, m.ld, e); };
+  Packer pk;
+  const Mat x = pk.fit(ws, a.x, e, must_pack(a.x));
+  const Mat wg = pk.fit(ws, a.wg, e, must_pack(a.wg));
+  const Mat wu = pk.fit(ws, a.wu, e, must_pack(a.wu));
+  const Mat wd = pk.fit(ws, a.wd, e, must_pack(a.wd));
+  const long long h_ld = round_up(1ll * a.f * e, 16) / e;
+  void* h = ws.take(static_cast<size_t>(h_ld) * a.rows * e);
+  const int kblock = 128 / e;
+
+  NarrowTask t1;
+  t1.a[0] = x; t1.a[1] = Mat{nullptr, 0, 0, 0};
+  t1.b[0] = wg; t1.b[1] = wu;
+  t1.m = a.rows; t1.n = a.f; t1.k = a.d;
+  t1.out[0] = h; t1.out[1] = const_cast<void*>(a.gate.p); t1.out[2] = const_cast<void*>(a.up.p);
+  t1.out_ld[0] = h_ld; t1.out_ld[1] = t1.out_ld[2] = a.f;
+  NarrowTask t2;
+  t2.a[0] = Mat{h, h_ld, a.rows, a.f}; t2.a[1] = Mat{nullptr, 0, 0, 0};
+  t2.b[0] = wd; t2.b[1] = Mat{nullptr, 0, 0, 0};
+  t2.m = a.rows; t2.n = a.d; t2.k = a.f;
+  t2.out[0] = a.y; t2.out_ld[0] = a.d;
+  const int cl = clusters_of(st);
+  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, true, false);
+  const NarrowPlan p2 = plan_narrow(&t2, 1, kblock, cl, false, true);
+  reserve_partials(ws, &t2, 1);
+  if (dry) return 0;
+  if (!ws.fits()) return -1;
+  if (pk.launch(s) != 0) return -1;
+  NarrowLaunch l{a.t, a.t.code, fnn::kEpiGated, a.act};
+  if (launch_pair(st, l, &t1, 1, p1, s) != 0) return -1;
+  l.epi = fnn::kEpiStore;
+  return launch_pair(st, l, &t2, 1, p2, s);
+}
+
+int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cudaStream_t s) {
+  const int e = a.t.bytes;
+  const bool dry = ws.dry;
+  auto must_pack = [&](const Mat& m) { return dry ? pack_all || ((m.ld * e) & 15) != 0 : !rows_addressable(m.p, m.ld, e); };
+  Packer pk;
+  const Mat dy = pk.fit(ws, a.dy, e, must_pack(a.dy));
+  const Mat x = pk.fit(ws, a.x, e, must_pack(a.x));
+  const Mat wg = pk.fit(ws, a.wg, e, must_pack(a.wg));
+  const Mat wu = pk.fit(ws, a.wu, e, must_pack(a.wu));
+  const Mat wd = pk.fit(ws, a.wd, e, must_pack(a.wd));
+  const bool pack_aux = must_pack(a.gate) || must_pack(a.up);     // one stride for both
+  const Mat gate = pk.fit(ws, a.gate, e, pack_aux);
+  const Mat up = pk.fit(ws, a.up, e, pack_aux);
+  const long long h_ld = round_up(1ll * a.f * e, 16) / e;
+  const size_t h_bytes = static_cast<size_t>(h_ld) * a.rows * e;
+  void* dg = ws.take(h_bytes);
+  void* du = ws.take(h_bytes);
+  void* h = ws.take(h_bytes);
+  const int kblock = 128 / e;
+  const Mat none{nullptr, 0, 0, 0};
+  const Mat mdg{dg, h_ld, a.rows, a.f}, mdu{du, h_ld, a.rows, a.f}, mh{h, h_ld, a.rows, a.f};
+
+  NarrowTask t1;                                   // dh = dy . Wd, never stored
+  t1.a[0] = dy; t1.a[1] = none; t1.b[0] = wd; t1.b[1] = none;
+  t1.b_mn = true;
+  t1.m = a.rows; t1.n = a.f; t1.k = a.d;
+  t1.out[0] = dg; t1.out[1] = du; t1.out[2] = h;
+  for (long long& ld : t1.out_ld) ld = h_ld;
+  t1.gate = gate.p; t1.up = up.p; t1.aux_ld = gate.ld;
+
+  NarrowTask g[4];
+  g[0].a[0] = mdg; g[0].a[1] = mdu; g[0].b[0] = wg; g[0].b[1] = wu;       // dx
+  g[0].b_mn = true;
+  g[0].m = a.rows; g[0].n = a.d; g[0].k = a.f; g[0].k2 = a.f;
+  g[0].out[0] = a.dx; g[0].out_ld[0] = a.d;
+  for (int i = 1; i <= 2; ++i) {                                          // dWg, dWu
+    g[i].a[0] = i == 1 ? mdg : mdu; g[i].a[1] = none; g[i].b[0] = x; g[i].b[1] = none;
+    g[i].a_mn = g[i].b_mn = true;
+    g[i].m = a.f; g[i].n = a.d; g[i].k = a.rows;
+    g[i].out[0] = i == 1 ? a.dwg : a.dwu; g[i].out_ld[0] = a.d;
+  }
+  g[3].a[0] = dy; g[3].a[1] = none; g[3].b[0] = mh; g[3].b[1] = none;     // dWd
+  g[3].a_mn = g[3].b_mn = true;
+  g[3].m = a.d; g[3].n = a.f; g[3].k = a.rows;
+  g[3].out[0] = a.dwd; g[3].out_ld[0] = a.f;
+  const int cl = clusters_of(st);
+  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, false, false);
+  const NarrowPlan p2 = plan_narrow(g, 4, kblock, cl, false, true);
+  reserve_partials(ws, g, 4);
+  if (dry) return 0;
+  if (!ws.fits()) return -1;
+  if (pk.launch(s) != 0) return -1;
+  NarrowLaunch l{a.t, a.t.code, fnn::kEpiGatedGrad, a.act};
+  if (launch_pair(st, l, &t1, 1, p1, s) != 0) return -1;
+  l.epi = fnn::kEpiStore;
+  return launch_pair(st, l, g, 4, p2, s);
+}
+
+bool ffn_sizes_ok(int rows, int d, int f) { return rows >= 0 && d >= 1 && f >= 1; }
+
+FfnArgs ffn_shape(const DType& t, int rows, int d, int f) {
+  FfnArgs a;
+  a.t = t; a.rows = rows; a.d = d; a.f = f; a.act = 0;
+  a.x = Mat{nullptr, d, rows, d};
+  a.dy = a.x;
+  a.wg = Mat{nullptr, d, f, d}; a.wu = a.wg;
+  a.wd = Mat{nullptr, f, d, f};
+  a.gate = Mat{nullptr, f, rows, f}; a.up = a.gate;
+  return a;
+}
+
+// ------------------------------------------------------------------ 8-bit products ---
+struct Int8Args {
+  Mat x, w, w2;              // w2: the up weight, or null
+  const float *xs, *ws, *ws2, *bias;
+  void* y;
+  int out_code, rows, k, n, act;
+  bool gated;
+};
+
+int int8_product(DeviceState* st, const Int8Args& a, Carver& ws, bool pack_all, cudaStream_t s) {
+  const bool dry = ws.dry;
+  auto must_pack = [&](const Mat& m) { return dry ? pack_all || (m.ld & 15) != 0 : !rows_addressable(m.p, m.ld, 1); };
+  Packer pk;
+  NarrowTask t;
+  t.a[0] = pk.fit(ws, a.x, 1, must_pack(a.x)); t.a[1] = Mat{nullptr, 0, 0, 0};
+  t.b[0] = pk.fit(ws, a.w, 1, must_pack(a.w));
+  t.b[1] = a.gated ? pk.fit(ws, a.w2, 1, must_pack(a.w2)) : Mat{nullptr, 0, 0, 0};
+  t.m = a.rows; t.n = a.n; t.k = a.k;
+  t.out[0] = a.y; t.out_ld[0] = a.n;
+  const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), a.gated, false);
+  if (dry) return 0;
+  if (!ws.fits()) return -1;
+  if (pk.launch(s) != 0) return -1;
+  NarrowLaunch l{kInt8, a.out_code, a.gated ? fnn::kEpiScaledGated : fnn::kEpiScaled, a.act};
+  l.row_scale = a.xs; l.col_scale = a.ws; l.col_scale2 = a.ws2; l.bias = a.bias;
+  return launch_pair(st, l, &t, 1, p, s);
+}
+
+// INT32 accumulators hold sums of k products of magnitude at most 128 * 128.
+constexpr int kInt8MaxK = 131071;
+
+template <typename T>
+int quantize_launch(const void* x, long long ld, int8_t* q, float* scale, int rows, int cols, cudaStream_t s) {
+  using namespace fnn;
+  const int v = 16 / static_cast<int>(sizeof(T));
+  const bool vec = rows_addressable(x, ld, sizeof(T)) && cols % v == 0 && (reinterpret_cast<uintptr_t>(q) & (v - 1)) == 0;
+  const T* src = static_cast<const T*>(x);
+  // a warp holds 32 * kQuantHeld vectors of a row; longer rows take a block each
+  const bool warp = cols <= 32 * kQuantHeld * v;
+  const int per = kQuantThreads / 32;
+  const int grid = warp ? (rows + per - 1) / per : rows;
+  if (warp && vec) quantize_rows_kernel<T, 32, true><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
+  else if (warp) quantize_rows_kernel<T, 32, false><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
+  else if (vec) quantize_rows_kernel<T, kQuantThreads, true><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
+  else quantize_rows_kernel<T, kQuantThreads, false><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  FNN_CUDA_OK(cudaGetLastError());
+  return 0;
+}
+
+}  // namespace
+
+extern "C" size_t fastnn_b200_gated_ffn_workspace(int dtype, int rows, int d_model, int d_ff, int backward,
+                                                  int unaligned) {
+  DType t;
+  if (!dtype_of(dtype, &t) || !ffn_sizes_ok(rows, d_model, d_ff)) return 0;
+  Carver ws{nullptr, 0, true};
+  const FfnArgs a = ffn_shape(t, rows, d_model, d_ff);
+  if (backward) ffn_backward(current_state(), a, ws, unaligned != 0, nullptr);
+  else ffn_forward(current_state(), a, ws, unaligned != 0, nullptr);
+  return ws.used;
+}
+
+extern "C" int fastnn_b200_gated_ffn_forward(int dtype, const void* x, long long ld_x, const void* w_gate,
+                                             const void* w_up, const void* w_down, void* y, void* gate, void* up,
+                                             int rows, int d_model, int d_ff, int act, void* workspace,
+                                             size_t workspace_bytes, void* stream) {
+  DType t;
+  if (!dtype_of(dtype, &t) || !ffn_sizes_ok(rows, d_model, d_ff) || !gate_act_ok(act) || ld_x < d_model) return -1;
+  if ((gate == nullptr) != (up == nullptr)) return -1;
+  if (rows == 0) return 0;
+  if (x == nullptr || w_gate == nullptr || w_up == nullptr || w_down == nullptr || y == nullptr) return -1;
+  DeviceState* st = current_state();
+  if (st == nullptr) return -1;
+  FfnArgs a = ffn_shape(t, rows, d_model, d_ff);
+  a.act = act;
+  a.x.p = x; a.x.ld = ld_x;
+  a.wg.p = w_gate; a.wu.p = w_up; a.wd.p = w_down;
+  a.gate.p = gate; a.up.p = up;
+  a.y = y;
+  Carver ws{static_cast<uint8_t*>(workspace), workspace_bytes, false};
+  return ffn_forward(st, a, ws, false, static_cast<cudaStream_t>(stream));
+}
+
+extern "C" int fastnn_b200_gated_ffn_backward(int dtype, const void* dy, long long ld_dy, const void* x, long long ld_x,
+                                              const void* gate, const void* up, const void* w_gate, const void* w_up,
+                                              const void* w_down, void* dx, void* dw_gate, void* dw_up, void* dw_down,
+                                              int rows, int d_model, int d_ff, int act, void* workspace,
+                                              size_t workspace_bytes, void* stream) {
+  DType t;
+  if (!dtype_of(dtype, &t) || !ffn_sizes_ok(rows, d_model, d_ff) || !gate_act_ok(act)) return -1;
+  if (ld_x < d_model || ld_dy < d_model) return -1;
+  if (dw_gate == nullptr || dw_up == nullptr || dw_down == nullptr) return -1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (rows == 0) {                                   // no tokens: the weights' gradients are zero
+    const size_t bytes = static_cast<size_t>(d_model) * d_ff * t.bytes;
+    void* outs[3] = {dw_gate, dw_up, dw_down};
+    for (void* o : outs) FNN_CUDA_OK(cudaMemsetAsync(o, 0, bytes, s));
+    return 0;
+  }
+  if (dy == nullptr || x == nullptr || gate == nullptr || up == nullptr || w_gate == nullptr || w_up == nullptr ||
+      w_down == nullptr || dx == nullptr)
+    return -1;
+  DeviceState* st = current_state();
+  if (st == nullptr) return -1;
+  FfnArgs a = ffn_shape(t, rows, d_model, d_ff);
+  a.act = act;
+  a.x.p = x; a.x.ld = ld_x;
+  a.dy.p = dy; a.dy.ld = ld_dy;
+  a.wg.p = w_gate; a.wu.p = w_up; a.wd.p = w_down;
+  a.gate.p = gate; a.up.p = up;
+  a.dx = dx; a.dwg = dw_gate; a.dwu = dw_up; a.dwd = dw_down;
+  Carver ws{static_cast<uint8_t*>(workspace), workspace_bytes, false};
+  return ffn_backward(st, a, ws, false, s);
+}
+
+extern "C" int fastnn_b200_quantize_rows(int dtype, const void* x, long long ld_x, signed char* q, float* scale,
+                                         int rows, int cols, void* stream) {
+  DType t;
+  if (!dtype_of(dtype, &t) || rows < 0 || cols < 1 || ld_x < cols) return -1;
+  if (rows == 0) return 0;
+  if (x == nullptr || q == nullptr || scale == nullptr || current_state() == nullptr) return -1;
+  cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (dtype == FASTNN_B200_F32) return quantize_launch<float>(x, ld_x, q, scale, rows, cols, s);
+  if (dtype == FASTNN_B200_F16) return quantize_launch<__half>(x, ld_x, q, scale, rows, cols, s);
+  return quantize_launch<__nv_bfloat16>(x, ld_x, q, scale, rows, cols, s);
+}
+
+namespace {
+int int8_entry(Int8Args a, void* workspace, size_t workspace_bytes, void* stream) {
+  DType t;
+  if (!dtype_of(a.out_code, &t) || a.rows < 0 || a.k < 1 || a.n < 1 || a.k > kInt8MaxK || !gate_act_ok(a.act)) return -1;
+  if (a.rows == 0) return 0;
+  if (a.x.p == nullptr || a.w.p == nullptr || a.xs == nullptr || a.ws == nullptr || a.y == nullptr) return -1;
+  if (a.gated && (a.w2.p == nullptr || a.ws2 == nullptr)) return -1;
+  DeviceState* st = current_state();
+  if (st == nullptr) return -1;
+  Carver ws{static_cast<uint8_t*>(workspace), workspace_bytes, false};
+  return int8_product(st, a, ws, false, static_cast<cudaStream_t>(stream));
+}
+Int8Args int8_shape(int rows, int k, int n, bool gated) {
+  Int8Args a;
+  std::memset(static_cast<void*>(&a), 0, sizeof(a));
+  a.x = Mat{nullptr, k, rows, k};
+  a.w = Mat{nullptr, k, n, k};
+  a.w2 = a.w;
+  a.rows = rows; a.k = k; a.n = n; a.gated = gated;
+  return a;
+}
+}  // namespace
+
+extern "C" size_t fastnn_b200_int8_workspace(int rows, int in_features, int out_features, int gated, int unaligned) {
+  if (rows < 0 || in_features < 1 || out_features < 1) return 0;
+  Carver ws{nullptr, 0, true};
+  int8_product(current_state(), int8_shape(rows, in_features, out_features, gated != 0), ws, unaligned != 0, nullptr);
+  return ws.used;
+}
+
+extern "C" int fastnn_b200_int8_linear_forward(const signed char* xq, const float* x_scale, const signed char* wq,
+                                               const float* w_scale, const float* bias, void* y, int out_dtype,
+                                               int rows, int in_features, int out_features, int act, void* workspace,
+                                               size_t workspace_bytes, void* stream) {
+  Int8Args a = int8_shape(rows, in_features, out_features, false);
+  a.x.p = xq; a.xs = x_scale; a.w.p = wq; a.ws = w_scale; a.bias = bias;
+  a.y = y; a.out_code = out_dtype; a.act = act;
+  return int8_entry(a, workspace, workspace_bytes, stream);
+}
+
+extern "C" int fastnn_b200_int8_gated_forward(const signed char* xq, const float* x_scale, const signed char* wq_gate,
+                                              const float* gate_scale, const signed char* wq_up, const float* up_scale,
+                                              void* h, int out_dtype, int rows, int in_features, int out_features,
+                                              int act, void* workspace, size_t workspace_bytes, void* stream) {
+  Int8Args a = int8_shape(rows, in_features, out_features, true);
+  a.x.p = xq; a.xs = x_scale; a.w.p = wq_gate; a.ws = gate_scale; a.w2.p = wq_up; a.ws2 = up_scale;
+  a.y = h; a.out_code = out_dtype; a.act = act;
+  return int8_entry(a, workspace, workspace_bytes, stream);
+}

@@ -88,6 +88,14 @@ FASTNN_B200_API int fastnn_cuda_matmul_batched_tn(const float* a, const float* b
 #define FASTNN_B200_ACT_RELU 1   /* max(x, 0)                   -- FastNN src/tensor/ops.rs:191-198 */
 #define FASTNN_B200_ACT_GELU 2   /* 0.5 x (1 + erf(x / sqrt 2)) -- FastNN src/tensor/ops.rs:220-230 */
 
+/* x / (1 + e^-x); the gated and 8-bit entries only */
+#define FASTNN_B200_ACT_SILU 5
+
+/* element types of the gated feed-forward and 8-bit entries */
+#define FASTNN_B200_F32 0
+#define FASTNN_B200_F16 1
+#define FASTNN_B200_BF16 2
+
 /* General form behind every GEMM entry:
  *   C[b] = act( alpha * op(A[b]) . op(B[b]) + beta * C[b] + bias )      b in [0, batch)
  * lda/ldb/ldc are row strides in elements, stride_a/b/c are batch strides in elements,
@@ -322,6 +330,76 @@ FASTNN_B200_API int fastnn_b200_reduce_partials(const float* partials, float* c,
 FASTNN_B200_API int fastnn_b200_gemm_splitk_static(int layout, const float* a, const float* b,
                                                    float* c, int m, int n, int k, int split_k,
                                                    void* stream);
+
+/* Gated feed-forward block:
+ *   y[rows,d_model] = ( act(x . Wg^T) * (x . Wu^T) ) . Wd^T
+ * x [rows,d_model], Wg and Wu [d_ff,d_model], Wd [d_model,d_ff], weights as Linear stores them, all of one
+ * type: FASTNN_B200_F16, _BF16 (16-bit operands, FP32 accumulate) or _F32 (TF32 multiply, as every
+ * FP32 product of this library).  act: none, ReLU, GELU(erf) or SiLU.  x may be a row-strided view (ld_x
+ * elements, >= d_model); everything else is dense.  Both projections, the activation and the product
+ * are one launch, the second product another; only act(gate) * up reaches memory between them, rounded
+ * to the operands' type.  gate and up (both or neither NULL) receive x . Wg^T and x . Wu^T
+ * [rows,d_ff], which the backward pass takes.  FastNN has no gated block; this stands beside
+ * fastnn_b200_linear_forward (Linear + GELU, src/nn/linear.rs:55-88).
+ * rows = 0 is a call without work.  Rows whose stride is no multiple of 16 bytes, and unaligned
+ * bases, are served through copies in the workspace.
+ *
+ * The caller owns the workspace: fastnn_b200_gated_ffn_workspace gives its size for a call
+ * (unaligned != 0: some operand's base or ld_x * element size is no multiple of 16 bytes), 0 for bad
+ * arguments.  It must be 16-byte aligned, belongs to the call until the stream has run it, and holds
+ * nothing between calls. */
+FASTNN_B200_API size_t fastnn_b200_gated_ffn_workspace(int dtype, int rows, int d_model, int d_ff,
+                                                       int backward, int unaligned);
+FASTNN_B200_API int fastnn_b200_gated_ffn_forward(int dtype, const void* x, long long ld_x,
+                                                  const void* w_gate, const void* w_up,
+                                                  const void* w_down, void* y, void* gate, void* up,
+                                                  int rows, int d_model, int d_ff, int act,
+                                                  void* workspace, size_t workspace_bytes,
+                                                  void* stream);
+
+/* Its backward pass, from dy [rows,d_model] and the saved gate and up:
+ *   dh = dy . Wd;  dgate = dh * up * act'(gate);  dup = dh * act(gate);  h = act(gate) * up
+ *   dx = dgate . Wg + dup . Wu;  dWg = dgate^T . x;  dWu = dup^T . x;  dWd = dy^T . h
+ * One launch forms dh and turns it into dgate, dup and h in its epilogue (dh is never stored; the three
+ * are rounded to the operands' type, as operands of the products after them); a second launch holds all
+ * four products.  act'(0) = 0 for ReLU, as FastNN's ReluBackward.  Outputs are overwritten; sums run in
+ * a fixed order, so equal inputs give equal bits.  rows = 0: the weights' gradients are zeroed. */
+FASTNN_B200_API int fastnn_b200_gated_ffn_backward(int dtype, const void* dy, long long ld_dy,
+                                                   const void* x, long long ld_x, const void* gate,
+                                                   const void* up, const void* w_gate,
+                                                   const void* w_up, const void* w_down, void* dx,
+                                                   void* dw_gate, void* dw_up, void* dw_down, int rows,
+                                                   int d_model, int d_ff, int act, void* workspace,
+                                                   size_t workspace_bytes, void* stream);
+
+/* Rows of x [rows,cols] (any of the three types, row stride ld_x) in signed 8-bit integers with one
+ * FP32 scale a row:  top = max |x|;  scale = top / 127;  q = round to even(x * (127 / top)), in FP32.
+ * A row with top < 2^-100 is taken as zero (q = 0, scale = 0); a row that holds a NaN or an infinity
+ * gets q = 0 and scale = NaN, which makes that row of a product NaN and no other.  Quantises activations
+ * per token and, applied to a weight [out,in], weights per output channel. */
+FASTNN_B200_API int fastnn_b200_quantize_rows(int dtype, const void* x, long long ld_x, signed char* q,
+                                              float* scale, int rows, int cols, void* stream);
+
+/* Linear in 8-bit integers with a scale for each token and each output channel:
+ *   y[t,o] = act( x_scale[t] * w_scale[o] * sum_i xq[t,i] * wq[o,i] + bias[o] )
+ * xq [rows,in], wq [out,in], bias [out] FP32 or NULL, y [rows,out] of out_dtype.  The sum is exact
+ * (INT32; in_features <= 131071).  The gated form is the first half of a gated block:
+ *   h[t,o] = act( x_scale[t] * gate_scale[o] * (xq . Wg^T) ) * ( x_scale[t] * up_scale[o] * (xq . Wu^T) )
+ * Workspace as above (a size of 0 needs none). */
+FASTNN_B200_API size_t fastnn_b200_int8_workspace(int rows, int in_features, int out_features, int gated,
+                                                  int unaligned);
+FASTNN_B200_API int fastnn_b200_int8_linear_forward(const signed char* xq, const float* x_scale,
+                                                    const signed char* wq, const float* w_scale,
+                                                    const float* bias, void* y, int out_dtype, int rows,
+                                                    int in_features, int out_features, int act,
+                                                    void* workspace, size_t workspace_bytes,
+                                                    void* stream);
+FASTNN_B200_API int fastnn_b200_int8_gated_forward(const signed char* xq, const float* x_scale,
+                                                   const signed char* wq_gate, const float* gate_scale,
+                                                   const signed char* wq_up, const float* up_scale,
+                                                   void* h, int out_dtype, int rows, int in_features,
+                                                   int out_features, int act, void* workspace,
+                                                   size_t workspace_bytes, void* stream);
 
 /* Stream-ordered forms of fastnn_cuda_memcpy_h2d / _d2h (cuda/kernels.cu:79-88, which are
  * synchronous): the copy is enqueued on `stream` and the call returns.  With pinned host memory a
