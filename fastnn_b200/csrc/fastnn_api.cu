@@ -22,6 +22,7 @@
 #include "conv_wgrad_tcgen05.cuh"
 #include "conv_wgrad_slab_tcgen05.cuh"
 #include "narrow_gemm_tcgen05.cuh"
+#include "narrow_skinny_tcgen05.cuh"
 #include "quantize_rows.cuh"
 
 namespace {

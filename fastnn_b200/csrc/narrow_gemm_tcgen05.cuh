@@ -262,8 +262,9 @@ __device__ __forceinline__ void for_act(int act, const Body& body) {
   else body(std::integral_constant<int, kActNone>());
 }
 
+template <typename Params>
 __device__ __forceinline__ bool narrow_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag,
-                                            const NarrowParams& p, unsigned int code) {
+                                            const Params& p, unsigned int code) {
   if (ptx::mbar_try_wait(bar, parity)) return true;
   const long long t0 = clock64();
   int it = 0;

@@ -4,6 +4,7 @@
 
 namespace {
 
+constexpr size_t kSkinnySmem = 115712;     // half of an SM's 228 KiB, less the 1 KiB reserved per CTA
 constexpr int kDefaultClusters = 74;       // CTA pairs of a B200, for size queries without a device
 
 struct DType {
@@ -139,13 +140,13 @@ struct NarrowPlan {
 // block_n / 2 rows of B per CTA) 1 / 64 clock a byte; a unit costs about 2000 clocks beside its k-blocks
 // (pipeline fill, the drain of its accumulator at the end of a wave), and a K split the reduction's
 // bytes and launch.  Units go round robin over the pairs, so their sums are exact.
-NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool gated, bool may_split) {
+struct PlanChoice {
+  int block_n, len;          // len: k-blocks of a unit, at most
+};
+PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int clusters, bool gated, bool may_split) {
   int max_kb = 1;
-  for (int i = 0; i < count; ++i) {
-    t[i].num_kb1 = ceil_div(t[i].k, kblock);
-    t[i].num_kb = t[i].num_kb1 + (t[i].k2 > 0 ? ceil_div(t[i].k2, kblock) : 0);
+  for (int i = 0; i < count; ++i)
     if (t[i].num_kb > max_kb) max_kb = t[i].num_kb;
-  }
   double best = 1e300;
   int best_bn = 256, best_len = max_kb;
   // a CTA's half of an MN-major B tile is whole 128-byte chunks of N
@@ -185,6 +186,41 @@ NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool 
       if (cost < best) { best = cost; best_bn = bn; best_len = len; }
     }
   }
+  return PlanChoice{best_bn, best_len};
+}
+
+// The choice walks some ten thousand combinations; programs repeat a handful of shapes, so answers are
+// remembered by shape.
+NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool gated, bool may_split) {
+  struct Slot {
+    int key[24];
+    PlanChoice choice;
+    bool valid;
+  };
+  constexpr int kSlots = 512;
+  static Slot memo[kSlots];
+  static std::mutex memo_mutex;
+  int key[24] = {kblock, clusters, gated ? 1 : 0, may_split ? 1 : 0, count};
+  uint64_t h = 0x9E3779B97F4A7C15ull;
+  for (int i = 0; i < count; ++i) {
+    t[i].num_kb1 = ceil_div(t[i].k, kblock);
+    t[i].num_kb = t[i].num_kb1 + (t[i].k2 > 0 ? ceil_div(t[i].k2, kblock) : 0);
+    int* q = key + 5 + 4 * i;
+    q[0] = t[i].m; q[1] = t[i].n; q[2] = t[i].num_kb; q[3] = t[i].b_mn ? 1 : 0;
+  }
+  for (int v : key) h = (h ^ static_cast<uint32_t>(v)) * 0x100000001B3ull;
+  PlanChoice c;
+  {
+    std::lock_guard<std::mutex> lock(memo_mutex);
+    Slot& slot = memo[(h >> 24) % kSlots];
+    if (!slot.valid || std::memcmp(slot.key, key, sizeof(key)) != 0) {
+      slot.choice = choose_narrow(t, count, kblock, clusters, gated, may_split);
+      std::memcpy(slot.key, key, sizeof(key));
+      slot.valid = true;
+    }
+    c = slot.choice;
+  }
+  const int best_bn = c.block_n, best_len = c.len;
   for (int i = 0; i < count; ++i) {
     t[i].split = ceil_div(t[i].num_kb, best_len);
     t[i].kb_per_split = ceil_div(t[i].num_kb, t[i].split);
@@ -226,6 +262,29 @@ NarrowKernel pair_kernel(int kind, int epi, int out_code) {
   return nullptr;
 }
 
+typedef void (*SkinnyKernel)(fnn::SkinnyParams);
+SkinnyKernel skinny_kernel(int kind, int epi, int out_code) {
+  using namespace fnn;
+  if (kind == kKindF16) {
+    const bool bf = out_code == FASTNN_B200_BF16;
+    if (epi == kEpiStore) return bf ? &narrow_skinny_kernel<kKindF16, kEpiStore, __nv_bfloat16> : &narrow_skinny_kernel<kKindF16, kEpiStore, __half>;
+    if (epi == kEpiGated) return bf ? &narrow_skinny_kernel<kKindF16, kEpiGated, __nv_bfloat16> : &narrow_skinny_kernel<kKindF16, kEpiGated, __half>;
+  } else if (kind == kKindTf32) {
+    if (epi == kEpiStore) return &narrow_skinny_kernel<kKindTf32, kEpiStore, float>;
+    if (epi == kEpiGated) return &narrow_skinny_kernel<kKindTf32, kEpiGated, float>;
+  } else {
+    if (epi == kEpiScaled)
+      return out_code == FASTNN_B200_F32 ? &narrow_skinny_kernel<kKindI8, kEpiScaled, float>
+             : (out_code == FASTNN_B200_BF16 ? &narrow_skinny_kernel<kKindI8, kEpiScaled, __nv_bfloat16>
+                                             : &narrow_skinny_kernel<kKindI8, kEpiScaled, __half>);
+    if (epi == kEpiScaledGated)
+      return out_code == FASTNN_B200_F32 ? &narrow_skinny_kernel<kKindI8, kEpiScaledGated, float>
+             : (out_code == FASTNN_B200_BF16 ? &narrow_skinny_kernel<kKindI8, kEpiScaledGated, __nv_bfloat16>
+                                             : &narrow_skinny_kernel<kKindI8, kEpiScaledGated, __half>);
+  }
+  return nullptr;
+}
+
 // Called once per device by fastnn_cuda_init.
 int narrow_init() {
   const int codes[3] = {FASTNN_B200_F32, FASTNN_B200_F16, FASTNN_B200_BF16};
@@ -233,8 +292,11 @@ int narrow_init() {
     for (int epi = 0; epi <= 4; ++epi)
       for (int c : codes) {
         NarrowKernel k = pair_kernel(kind, epi, c);
-        if (k == nullptr) continue;
-        FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
+        if (k != nullptr)
+          FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
+        SkinnyKernel sk = skinny_kernel(kind, epi, c);
+        if (sk != nullptr)
+          FNN_CUDA_OK(cudaFuncSetAttribute(sk, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSkinnySmem)));
       }
   return 0;
 }
@@ -351,6 +413,94 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   return 0;
 }
 
+// Few tokens take the form with the weights on the M side; set_policy(4) keeps CTA pairs.
+bool use_skinny(int tokens) { return tokens <= fnn::kSkinnyMaxTokens && t_policy.policy != 4; }
+
+// K slices of a row tile (the CTAs of one cluster).
+int skinny_split(int tiles, int num_kb) {
+  int want = t_policy.split_k;
+  if (want == 0) {
+    want = 1;
+    while (want < 8 && tiles * want < 256) want *= 2;
+  }
+  int split = 8;
+  while (split > 1 && (split > want || num_kb < 2 * split)) split /= 2;
+  return split;
+}
+
+// Operands as launch_pair's; t.a[0] holds the tokens, t.b the weights.
+int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, bool early_w, cudaStream_t stream) {
+  using namespace fnn;
+  SkinnyParams p;
+  std::memset(&p, 0, sizeof(p));
+  const bool two = l.epi == kEpiGated || l.epi == kEpiScaledGated;
+  const int kblock = 128 / l.in.bytes;
+  const int tile_rows = two ? 64 : 128;
+  p.tokens = t.m; p.n = t.n;
+  p.n_mma = ceil_div(t.m, 16) * 16;
+  p.num_kb = ceil_div(t.k, kblock);
+  const int tiles = ceil_div(t.n, tile_rows);
+  p.split = skinny_split(tiles, p.num_kb);
+  bool ok = encode_narrow(&p.x, l.in, t.a[0].p, t.a[0].cols, t.a[0].rows, 1, t.a[0].ld * l.in.bytes,
+                          t.a[0].ld * l.in.bytes * t.a[0].rows, kblock, p.n_mma, false);
+  for (int j = 0; j < (two ? 2 : 1); ++j)
+    ok = ok && encode_narrow(&p.w[j], l.in, t.b[j].p, t.b[j].cols, t.b[j].rows, 1, t.b[j].ld * l.in.bytes,
+                             t.b[j].ld * l.in.bytes * t.b[j].rows, kblock, tile_rows, false);
+  if (!ok) return -1;
+  DType out;
+  if (!dtype_of(l.out_code, &out)) return -1;
+  for (int j = 0; j < 3; ++j) {
+    p.out[j] = t.out[j];
+    p.out_ld[j] = t.out_ld[j];
+    p.vec_out[j] = (reinterpret_cast<uintptr_t>(t.out[j]) % (4 * out.bytes) == 0 && t.out_ld[j] % 4 == 0) ? 1 : 0;
+  }
+  const int slice_kb = ceil_div(p.num_kb, p.split);
+  const size_t stage = kNarrowABytes + static_cast<size_t>(p.n_mma) * 128;
+  int stages = static_cast<int>((kSkinnySmem - skinny_smem_bytes(p.n_mma, 0)) / stage);
+  if (stages > kSkinnyMaxStages) stages = kSkinnyMaxStages;
+  if (stages > slice_kb) stages = slice_kb;
+  const int for_partial = static_cast<int>((p.n_mma * 512 + stage - 1) / stage);    // the ring holds the partial tile
+  if (stages < for_partial) stages = for_partial;
+  p.num_stages = stages;
+  p.tmem_cols = 32;
+  while (p.tmem_cols < p.n_mma) p.tmem_cols *= 2;
+  p.early_w = early_w ? 1 : 0;
+  p.act = l.act;
+  p.is_bf16 = l.in.code == FASTNN_B200_BF16 ? 1 : 0;
+  p.row_scale = l.row_scale; p.col_scale = l.col_scale; p.col_scale2 = l.col_scale2; p.bias = l.bias;
+  p.status = st->status;
+  p.spin_budget = st->spin_budget;
+  // Tensor memory is 512 columns: no more CTAs may share an SM than have their columns (a CTA that waits
+  // for columns while its cluster waits for it would never get them), which the shared memory enforces.
+  const size_t sm_smem = 228 * 1024;
+  const size_t floor_bytes = sm_smem / (512 / p.tmem_cols + 1) + 1;
+  size_t smem = skinny_smem_bytes(p.n_mma, stages);
+  if (smem < floor_bytes) smem = floor_bytes;
+  SkinnyKernel k = skinny_kernel(l.in.kind, l.epi, l.out_code);
+  if (k == nullptr || smem > kSkinnySmem) return -1;
+  const long long grid = 1ll * tiles * p.split;
+  if (grid > 0x7fffffffll) return -1;
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
+  cfg.blockDim = dim3(kSkinnyThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attrs[2];
+  attrs[0].id = cudaLaunchAttributeClusterDimension;
+  attrs[0].val.clusterDim.x = static_cast<unsigned>(p.split);
+  attrs[0].val.clusterDim.y = 1;
+  attrs[0].val.clusterDim.z = 1;
+  attrs[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attrs[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attrs;
+  cfg.numAttrs = tunables().pdl ? 2 : 1;
+  FNN_CUDA_OK(cudaLaunchKernelEx(&cfg, k, p));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  t_last = LastCall{13, p.n_mma, p.split, static_cast<int>(grid)};
+  return 0;
+}
+
 // ------------------------------------------------------------- gated feed-forward ---
 struct FfnArgs {
   DType t;
@@ -389,6 +539,16 @@ int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cu
   t2.b[0] = wd; t2.b[1] = Mat{nullptr, 0, 0, 0};
   t2.m = a.rows; t2.n = a.d; t2.k = a.f;
   t2.out[0] = a.y; t2.out_ld[0] = a.d;
+  NarrowLaunch l{a.t, a.t.code, fnn::kEpiGated, a.act};
+  if (use_skinny(a.rows)) {
+    if (dry) return 0;
+    if (!ws.fits()) return -1;
+    if (pk.launch(s) != 0 || launch_skinny(st, l, t1, false, s) != 0) return -1;
+    l.epi = fnn::kEpiStore;
+    // Wd may be read early: the launch ahead writes only h, gate and up, and has itself waited for
+    // whatever came before it
+    return launch_skinny(st, l, t2, true, s);
+  }
   const int cl = clusters_of(st);
   const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, true, false);
   const NarrowPlan p2 = plan_narrow(&t2, 1, kblock, cl, false, true);
@@ -396,7 +556,6 @@ int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cu
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
-  NarrowLaunch l{a.t, a.t.code, fnn::kEpiGated, a.act};
   if (launch_pair(st, l, &t1, 1, p1, s) != 0) return -1;
   l.epi = fnn::kEpiStore;
   return launch_pair(st, l, &t2, 1, p2, s);
@@ -492,12 +651,13 @@ int int8_product(DeviceState* st, const Int8Args& a, Carver& ws, bool pack_all, 
   t.b[1] = a.gated ? pk.fit(ws, a.w2, 1, must_pack(a.w2)) : Mat{nullptr, 0, 0, 0};
   t.m = a.rows; t.n = a.n; t.k = a.k;
   t.out[0] = a.y; t.out_ld[0] = a.n;
-  const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), a.gated, false);
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
   NarrowLaunch l{kInt8, a.out_code, a.gated ? fnn::kEpiScaledGated : fnn::kEpiScaled, a.act};
   l.row_scale = a.xs; l.col_scale = a.ws; l.col_scale2 = a.ws2; l.bias = a.bias;
+  if (use_skinny(a.rows)) return launch_skinny(st, l, t, false, s);
+  const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), a.gated, false);
   return launch_pair(st, l, &t, 1, p, s);
 }
 

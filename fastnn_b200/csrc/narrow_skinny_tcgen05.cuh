@@ -1,0 +1,312 @@
+// The same products for few tokens (decoding): the weight's rows on the tensor core's M side.
+//
+//   out[t, r] = epilogue( sum_k x[t, k] * W[r, k] )        t < tokens <= 128
+//
+// With up to 128 tokens the time is that of reading the weights once, so the form is chosen for bytes in
+// flight and for even shares of them.  A CTA takes 128 rows of W (a gated product: 64 rows of the gate's
+// weight and the same 64 of the up projection's) and one slice of K, and streams them through a ring of
+// TMA stages; the tokens are the MMA's N (rounded up to 16, rows past the last one read as zero), so one
+// tcgen05.mma per 32 bytes of K covers all of them and the tensor core is never what is waited for.
+// The slices of a row tile are the CTAs of one cluster: each leaves its accumulator in its own shared
+// memory as [token][row], and after a cluster barrier the CTAs add the slices in ascending order over
+// distributed shared memory, apply the epilogue and write -- no workspace, no second kernel, the same
+// bits every time.  A CTA asks for at most half of an SM, so that a CTA's start and end lie under its
+// neighbour's stream, and so that the next kernel's CTAs find room while this one's last are running.
+#pragma once
+#include "narrow_gemm_tcgen05.cuh"
+
+namespace fnn {
+
+constexpr int kSkinnyMaxTokens = 128;
+constexpr int kSkinnyThreads = 192;                 // producer, MMA issuer, four warps that drain the accumulator
+constexpr int kSkinnyMaxStages = 8;
+constexpr int kSkinnyBarBytes = 256;
+
+struct SkinnyParams {
+  CUtensorMap w[2], x;
+  void* out[3];              // as NarrowProblem: the product, and for a gated one optionally gate and up
+  long long out_ld[3];
+  int vec_out[3];            // rows may be written four columns at a time
+  int tokens, n;             // n: columns of one output
+  int n_mma;                 // tokens rounded up to 16
+  int num_kb, split, num_stages, tmem_cols;
+  int early_w;               // the weights may be read before the kernel ahead of this one has finished
+  int act, is_bf16;
+  const float* row_scale;
+  const float* col_scale;
+  const float* col_scale2;
+  const float* bias;
+  unsigned int* status;
+  long long spin_budget;
+};
+
+namespace ptx {
+template <int kKind>
+__device__ __forceinline__ void mma_narrow_1cta(uint32_t tmem_d, uint64_t desc_a, uint64_t desc_b, uint32_t idesc,
+                                                uint32_t accumulate) {
+  if constexpr (kKind == kKindF16)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+                 "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+  else if constexpr (kKind == kKindI8)
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+                 "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
+                 "l"(desc_a), "l"(desc_b), "r"(idesc), "r"(accumulate)
+                 : "memory");
+  else
+    mma_tf32_1cta(tmem_d, desc_a, desc_b, idesc, accumulate);
+}
+// This warp's 32 lanes x 16 consecutive 32-bit columns.
+__device__ __forceinline__ void tmem_ld_32x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
+}  // namespace ptx
+
+// Four sums over the slices of one token's consecutive rows.
+template <int kKind>
+__device__ __forceinline__ void skinny_sum(uint32_t local, int split, float (&v)[4]) {
+  if constexpr (kKind == kKindI8) {
+    int s[4] = {0, 0, 0, 0};
+    for (int r = 0; r < split; ++r) {
+      const float4 t = ptx::ld_shared_cluster_f4(ptx::mapa_shared(local, static_cast<uint32_t>(r)));
+      s[0] += __float_as_int(t.x); s[1] += __float_as_int(t.y); s[2] += __float_as_int(t.z); s[3] += __float_as_int(t.w);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = static_cast<float>(s[j]);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = 0.0f;
+    for (int r = 0; r < split; ++r) {
+      const float4 t = ptx::ld_shared_cluster_f4(ptx::mapa_shared(local, static_cast<uint32_t>(r)));
+      v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ void skinny_put(void* out, long long ld, int vec, int t, int c, int n, const float (&v)[4]) {
+  T* dst = static_cast<T*>(out) + static_cast<long long>(t) * ld + c;
+  if (vec && c + 4 <= n) {
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+    else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c + j < n) dst[j] = static_cast<T>(v[j]);
+  }
+}
+
+template <int kKind, int kEpi, typename OutT>
+__global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __grid_constant__ SkinnyParams p) {
+  using K = NarrowKind<kKind>;
+  constexpr bool kTwo = kEpi == kEpiGated || kEpi == kEpiScaledGated;
+  constexpr int kRows = kTwo ? 64 : 128;              // output columns of a tile
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
+  const uint32_t x_bytes = static_cast<uint32_t>(p.n_mma) * 128u;
+  const uint32_t stage_bytes = kNarrowABytes + x_bytes;       // x_bytes is a multiple of 2048
+  const uint32_t bar_base = smem_base + p.num_stages * stage_bytes;
+  uint8_t* bar_gen = smem_gen + (bar_base - smem_base);
+  auto full_bar = [&](int s) { return bar_base + 8u * s; };
+  auto empty_bar = [&](int s) { return bar_base + 64u + 8u * s; };
+  const uint32_t done_bar = bar_base + 128u;
+  const uint32_t tmem_slot = bar_base + 136u;
+  volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(bar_gen + 136);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 140);
+
+  const int slice = static_cast<int>(blockIdx.x) % p.split;   // = rank in the cluster
+  const int tile = static_cast<int>(blockIdx.x) / p.split;
+  const int r0 = tile * kRows;
+  const int kb0 = static_cast<int>(static_cast<long long>(slice) * p.num_kb / p.split);
+  const int kb1 = static_cast<int>(static_cast<long long>(slice + 1) * p.num_kb / p.split);
+
+  auto load_w = [&](int kb, int s, uint64_t pol) {
+    const uint32_t sa = smem_base + s * stage_bytes;
+    const uint32_t fb = full_bar(s);
+    ptx::mbar_expect_tx(fb, stage_bytes);
+    if constexpr (kTwo) {
+      ptx::tma_load_3d_hint(sa, &p.w[0], fb, kb * K::kBlock, r0, 0, pol);
+      ptx::tma_load_3d_hint(sa + 64 * 128, &p.w[1], fb, kb * K::kBlock, r0, 0, pol);
+    } else {
+      ptx::tma_load_3d_hint(sa, &p.w[0], fb, kb * K::kBlock, r0, 0, pol);
+    }
+  };
+  auto load_x = [&](int kb, int s) {
+    ptx::tma_load_3d(smem_base + s * stage_bytes + kNarrowABytes, &p.x, full_bar(s), kb * K::kBlock, 0, 0);
+  };
+
+  int pre = 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.num_stages; ++s) {
+      ptx::mbar_init(full_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), 1);
+    }
+    ptx::mbar_init(done_bar, 1);
+    *abort_flag = 0;
+    ptx::fence_mbar_init();
+    ptx::fence_proxy_async_smem();
+    const uint64_t pol = ptx::make_l2_policy(3);
+    pre = min(p.num_stages, kb1 - kb0);
+    // weights that nothing ahead in the stream can still be writing start before that kernel has ended
+    if (!p.early_w) ptx::grid_dep_wait();
+    for (int i = 0; i < pre; ++i) load_w(kb0 + i, i, pol);
+    if (p.early_w) ptx::grid_dep_wait();
+    for (int i = 0; i < pre; ++i) load_x(kb0 + i, i);
+  }
+  if (warp == 1) {
+    ptx::tmem_alloc_1cta(tmem_slot, static_cast<uint32_t>(p.tmem_cols));
+    ptx::tmem_relinquish_1cta();
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  ptx::tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot_gen;
+  // The next kernel's CTAs may come once every CTA of this grid holds its tensor memory and has seen the
+  // kernels before it finish (thread 0 waited above): what the next kernel reads early is then final.
+  ptx::grid_dep_launch_dependents();
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol = ptx::make_l2_policy(3);
+      int stage = pre % p.num_stages;
+      uint32_t phase = pre == p.num_stages ? 1u : 0u;
+      for (int kb = kb0 + pre; kb < kb1; ++kb) {
+        if (!narrow_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, kStatusProducerTimeout)) break;
+        load_w(kb, stage, pol);
+        load_x(kb, stage);
+        if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      const uint32_t idesc = ptx::idesc_narrow<kKind>(128, p.n_mma, 0, 0, p.is_bf16);
+      const uint64_t a_desc0 = narrow_desc<kKind>(smem_base, 0);
+      const uint64_t b_desc0 = narrow_desc<kKind>(smem_base + kNarrowABytes, 0);
+      const uint64_t stage_step = stage_bytes >> 4;
+      int stage = 0;
+      uint32_t phase = 0;
+      uint32_t accumulate = 0u;
+      bool ok = true;
+      for (int kb = kb0; kb < kb1; ++kb) {
+        ok = narrow_wait(full_bar(stage), phase, abort_flag, p, kStatusMmaTimeout);
+        if (!ok) break;
+        const uint64_t da = a_desc0 + stage * stage_step;
+        const uint64_t db = b_desc0 + stage * stage_step;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) {
+          ptx::mma_narrow_1cta<kKind>(tmem_base, da + ks * 2, db + ks * 2, idesc, accumulate);
+          accumulate = 1u;
+        }
+        ptx::mma_commit_1cta(empty_bar(stage));
+        if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
+      }
+      if (ok) ptx::mma_commit_1cta(done_bar);
+    }
+  } else {
+    // The accumulator to shared memory as [token][row], over the ring: every stage has been consumed.
+    bool ok = narrow_wait(done_bar, 0u, abort_flag, p, kStatusEpilogueTimeout);
+    ok = __all_sync(0xffffffffu, ok);
+    if (ok) {
+      ptx::tc_fence_after_sync();
+      const int q = warp & 3;
+      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
+      uint32_t* part = reinterpret_cast<uint32_t*>(smem_gen) + q * 32 + lane;
+      for (int c = 0; c < p.n_mma; c += 16) {
+        uint32_t r[16];
+        ptx::tmem_ld_32x16(taddr + c, r);
+        ptx::tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) part[(c + j) * 128] = r[j];
+      }
+      ptx::tc_fence_before_sync();
+    }
+  }
+
+  // Every thread of every CTA of the cluster passes both barriers, aborting or not.
+  ptx::grid_dep_wait();                               // before any thread reads or writes other global data
+  __syncwarp();
+  ptx::cluster_arrive_release();
+  ptx::cluster_wait_acquire();
+  if (!*abort_flag) {
+    constexpr int kQuads = kRows / 4;
+    const int total = p.tokens * kQuads;
+    for (int i = slice * kSkinnyThreads + static_cast<int>(threadIdx.x); i < total; i += p.split * kSkinnyThreads) {
+      const int t = i / kQuads;
+      const int r = (i - t * kQuads) * 4;
+      const int c = r0 + r;
+      if (c >= p.n) continue;
+      const uint32_t local = smem_base + static_cast<uint32_t>(t * 128 + r) * 4u;
+      float v[4];
+      skinny_sum<kKind>(local, p.split, v);
+      if constexpr (kEpi == kEpiStore) {
+        skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
+      } else if constexpr (kEpi == kEpiGated) {
+        float u[4];
+        skinny_sum<kKind>(local + 64 * 4, p.split, u);
+        if (p.out[1] != nullptr) {
+          skinny_put<OutT>(p.out[1], p.out_ld[1], p.vec_out[1], t, c, p.n, v);
+          skinny_put<OutT>(p.out[2], p.out_ld[2], p.vec_out[2], t, c, p.n, u);
+        }
+        for_act(p.act, [&](auto tag) {
+          constexpr int kAct = decltype(tag)::value;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] = gate_act<kAct>(v[j]) * u[j];
+        });
+        skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
+      } else {
+        const float rs = __ldg(p.row_scale + t);
+        float cs[4], more[4], u[4];
+        if constexpr (kEpi == kEpiScaledGated) skinny_sum<kKind>(local + 64 * 4, p.split, u);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool in = c + j < p.n;
+          cs[j] = in ? __ldg(p.col_scale + c + j) : 0.0f;
+          if constexpr (kEpi == kEpiScaledGated) more[j] = in ? __ldg(p.col_scale2 + c + j) : 0.0f;
+          else more[j] = in && p.bias != nullptr ? __ldg(p.bias + c + j) : 0.0f;
+        }
+        for_act(p.act, [&](auto tag) {
+          constexpr int kAct = decltype(tag)::value;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            if constexpr (kEpi == kEpiScaledGated)
+              v[j] = gate_act<kAct>(v[j] * (rs * cs[j])) * (u[j] * (rs * more[j]));
+            else
+              v[j] = gate_act<kAct>(fmaf(v[j], rs * cs[j], more[j]));
+          }
+        });
+        skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
+      }
+    }
+  }
+  __syncwarp();
+  ptx::cluster_arrive_release();                      // no CTA leaves while its shared memory is being read
+  ptx::cluster_wait_acquire();
+
+  if (*abort_flag) {
+    const long long t0 = clock64();
+    while (clock64() - t0 < 2000000) { }
+  }
+  ptx::tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    ptx::tc_fence_after_sync();
+    ptx::tmem_dealloc_1cta(tmem_base, static_cast<uint32_t>(p.tmem_cols));
+  }
+}
+
+inline size_t skinny_smem_bytes(int n_mma, int num_stages) {
+  return 1024 + static_cast<size_t>(num_stages) * (kNarrowABytes + n_mma * 128) + kSkinnyBarBytes;
+}
+
+}  // namespace fnn
