@@ -339,72 +339,62 @@ _DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
 _GATE_ACTS = (ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU)
 
 
-def _on_stream(stream, call):
-    """``call(raw stream)`` with torch's current stream set to the one the kernels run on."""
-    if stream is None:
-        return call(torch.cuda.current_stream().cuda_stream)
-    with torch.cuda.stream(torch.cuda.ExternalStream(int(stream))):
-        return call(int(stream))
+def _as_current(stream):
+    return torch.cuda.stream(torch.cuda.ExternalStream(int(stream)))
 
 
-def _rows_view(t, cols, name):
-    """(rows, row stride) of a tensor [.., cols] whose rows are contiguous and evenly spaced."""
-    if t.dim() < 1 or int(t.shape[-1]) != cols:
-        raise ValueError(f"{name}: expected {cols} features, got shape {tuple(t.shape)}")
-    rows = t.numel() // cols
+def _raw_stream(t):
+    """The current stream of the tensor's device as an integer (current_stream() without its objects)."""
+    return torch._C._cuda_getCurrentRawStream(t.get_device())
+
+
+def _row_stride(t, cols, name):
+    """Row stride of a tensor [.., cols] whose rows are contiguous and evenly spaced."""
     if t.is_contiguous():
-        return rows, cols
+        return cols
     if t.stride(-1) == 1 or cols == 1:
+        if t.numel() <= cols:
+            return cols
         try:
             ld = int(t.view(-1, cols).stride(0))
         except RuntimeError:
             ld = 0
-        if ld >= cols or rows <= 1:
-            return rows, max(ld, cols)
+        if ld >= cols:
+            return ld
     raise ValueError(f"{name}: rows must be contiguous, evenly spaced and not overlap")
 
 
 def _check_like(t, name, dtype, device, shape):
     if t.dtype != dtype or t.device != device or not t.is_contiguous():
         raise ValueError(f"{name}: expected a contiguous {dtype} tensor on {device}")
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name}: expected shape {shape}, got {tuple(t.shape)}")
+    if t.shape != shape:
+        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
 
 
-def _workspace(nbytes, device):
-    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
-
-
-def _unaligned(size, *tensors_and_strides):
-    """1 when some base or row stride (bytes) is no multiple of 16."""
-    bits = 0
-    for t, ld in tensors_and_strides:
-        bits |= t.data_ptr() | ld * size
-    return 1 if bits & 15 else 0
-
-
-def _new_out(shape, dtype, device, out):
+def _new_out(shape, dtype, like, out):
     if out is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    _check_like(out, "out", dtype, device, tuple(shape))
+        return like.new_empty(shape, dtype=dtype)
+    _check_like(out, "out", dtype, like.device, shape)
     return out
 
 
 def _ffn_shapes(x, w_gate, w_up, w_down, act):
-    if not x.is_cuda or x.dtype not in _DTYPE_CODE:
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None or not x.is_cuda or x.dim() < 1:
         raise ValueError("x: expected a float32, float16 or bfloat16 CUDA tensor")
     if act not in _GATE_ACTS:
         raise ValueError("act must be ACT_NONE, ACT_RELU, ACT_GELU or ACT_SILU")
-    if w_gate.dim() != 2:
-        raise ValueError("w_gate must be [d_ff, d_model]")
-    f, d = int(w_gate.shape[0]), int(w_gate.shape[1])
-    if f < 1 or d < 1:
-        raise ValueError("the block needs at least one feature on either side")
-    _check_like(w_gate, "w_gate", x.dtype, x.device, (f, d))
-    _check_like(w_up, "w_up", x.dtype, x.device, (f, d))
-    _check_like(w_down, "w_down", x.dtype, x.device, (d, f))
+    if w_gate.dim() != 2 or w_gate.numel() == 0:
+        raise ValueError("w_gate must be [d_ff, d_model], neither of them 0")
+    f, d = w_gate.shape
+    if x.shape[-1] != d:
+        raise ValueError(f"Expected input features {d}")
+    dtype, device = x.dtype, x.device
+    _check_like(w_gate, "w_gate", dtype, device, (f, d))
+    _check_like(w_up, "w_up", dtype, device, (f, d))
+    _check_like(w_down, "w_down", dtype, device, (d, f))
     _ensure_ctx(x)
-    return d, f
+    return code, d, f
 
 
 def gated_ffn_forward(x, w_gate, w_up, w_down, act=ACT_SILU, return_pre=False, out=None, stream=None):
@@ -412,51 +402,56 @@ def gated_ffn_forward(x, w_gate, w_up, w_down, act=ACT_SILU, return_pre=False, o
     w_down [d_model, d_ff] as Linear stores weights (two halves of one fused matrix will do); all bfloat16,
     all float16, or all float32 (TF32 multiply).  Both projections, the activation and the product are one
     launch.  With ``return_pre`` returns (y, gate, up): the projections gated_ffn_backward takes."""
-    d, f = _ffn_shapes(x, w_gate, w_up, w_down, act)
-    rows, ld = _rows_view(x, d, "x")
-    code, size = _DTYPE_CODE[x.dtype], x.element_size()
-    unaligned = _unaligned(size, (x, ld), (w_gate, 0), (w_up, 0), (w_down, 0))
-
-    def call(s):
-        y = _new_out(x.shape, x.dtype, x.device, out)
-        gate = up = None
-        if return_pre:
-            gate = torch.empty(*x.shape[:-1], f, dtype=x.dtype, device=x.device)
-            up = torch.empty_like(gate)
-        nbytes = lib().fastnn_b200_gated_ffn_workspace(code, rows, d, f, 0, unaligned)
-        ws = _workspace(nbytes, x.device)
-        if lib().fastnn_b200_gated_ffn_forward(code, _ptr(x), ld, _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(y),
-                                               _ptr(gate), _ptr(up), rows, d, f, act, _ptr(ws), nbytes, s) != 0:
-            raise CudaError("CUDA gated_ffn_forward failed")
-        return (y, gate, up) if return_pre else y
-    return _on_stream(stream, call)
+    if stream is not None:
+        with _as_current(stream):
+            return gated_ffn_forward(x, w_gate, w_up, w_down, act, return_pre, out)
+    code, d, f = _ffn_shapes(x, w_gate, w_up, w_down, act)
+    ld = _row_stride(x, d, "x")
+    rows = x.numel() // d
+    px, pg, pu, pd = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
+    unaligned = 1 if (px | pg | pu | pd | ld * x.element_size()) & 15 else 0
+    y = _new_out(x.shape, x.dtype, x, out)
+    gate = up = None
+    if return_pre:
+        gate = x.new_empty(x.shape[:-1] + (f,))
+        up = torch.empty_like(gate)
+    nbytes = lib().fastnn_b200_gated_ffn_workspace(code, rows, d, f, 0, unaligned)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    if lib().fastnn_b200_gated_ffn_forward(code, px, ld, pg, pu, pd, y.data_ptr(), gate.data_ptr() if return_pre else 0,
+                                           up.data_ptr() if return_pre else 0, rows, d, f, act, ws.data_ptr(), nbytes,
+                                           _raw_stream(x)) != 0:
+        raise CudaError("CUDA gated_ffn_forward failed")
+    return (y, gate, up) if return_pre else y
 
 
 def gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act=ACT_SILU, stream=None):
     """(dx, dw_gate, dw_up, dw_down) of gated_ffn_forward from dy [.., d_model], its input x and the saved
     gate and up [.., d_ff].  Equal inputs give equal bits."""
-    d, f = _ffn_shapes(x, w_gate, w_up, w_down, act)
-    rows, ld_x = _rows_view(x, d, "x")
+    if stream is not None:
+        with _as_current(stream):
+            return gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act)
+    code, d, f = _ffn_shapes(x, w_gate, w_up, w_down, act)
+    ld_x = _row_stride(x, d, "x")
+    rows = x.numel() // d
     if dy.dtype != x.dtype or dy.device != x.device or dy.shape != x.shape:
         raise ValueError("dy: expected a tensor like x")
-    _, ld_dy = _rows_view(dy, d, "dy")
-    saved = tuple(x.shape[:-1]) + (f,)
+    ld_dy = _row_stride(dy, d, "dy")
+    saved = x.shape[:-1] + (f,)
     _check_like(gate, "gate", x.dtype, x.device, saved)
     _check_like(up, "up", x.dtype, x.device, saved)
-    code, size = _DTYPE_CODE[x.dtype], x.element_size()
-    unaligned = _unaligned(size, (x, ld_x), (dy, ld_dy), (gate, 0), (up, 0), (w_gate, 0), (w_up, 0), (w_down, 0))
-
-    def call(s):
-        dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        dwg, dwu, dwd = torch.empty_like(w_gate), torch.empty_like(w_up), torch.empty_like(w_down)
-        nbytes = lib().fastnn_b200_gated_ffn_workspace(code, rows, d, f, 1, unaligned)
-        ws = _workspace(nbytes, x.device)
-        if lib().fastnn_b200_gated_ffn_backward(code, _ptr(dy), ld_dy, _ptr(x), ld_x, _ptr(gate), _ptr(up),
-                                                _ptr(w_gate), _ptr(w_up), _ptr(w_down), _ptr(dx), _ptr(dwg),
-                                                _ptr(dwu), _ptr(dwd), rows, d, f, act, _ptr(ws), nbytes, s) != 0:
-            raise CudaError("CUDA gated_ffn_backward failed")
-        return dx, dwg, dwu, dwd
-    return _on_stream(stream, call)
+    ptrs = [t.data_ptr() for t in (dy, x, gate, up, w_gate, w_up, w_down)]
+    bits = (ld_x | ld_dy) * x.element_size()
+    for p in ptrs:
+        bits |= p
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dwg, dwu, dwd = torch.empty_like(w_gate), torch.empty_like(w_up), torch.empty_like(w_down)
+    nbytes = lib().fastnn_b200_gated_ffn_workspace(code, rows, d, f, 1, 1 if bits & 15 else 0)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
+    if lib().fastnn_b200_gated_ffn_backward(code, ptrs[0], ld_dy, ptrs[1], ld_x, *ptrs[2:], dx.data_ptr(), dwg.data_ptr(),
+                                            dwu.data_ptr(), dwd.data_ptr(), rows, d, f, act, ws.data_ptr(), nbytes,
+                                            _raw_stream(x)) != 0:
+        raise CudaError("CUDA gated_ffn_backward failed")
+    return dx, dwg, dwu, dwd
 
 
 def quantize_rows(x, stream=None):
@@ -464,85 +459,95 @@ def quantize_rows(x, stream=None):
     float32 scale a row, scale = max|row| / 127 and q = round to even(row * (127 / max|row|)).  Rows below
     2**-100 count as zero; a row with a NaN or an infinity gets scale NaN.  For activations [.., in] the
     scales are per token, for a weight [out, in] per output channel."""
-    if not x.is_cuda or x.dtype not in _DTYPE_CODE:
-        raise ValueError("x: expected a float32, float16 or bfloat16 CUDA tensor")
-    if x.dim() < 1 or int(x.shape[-1]) < 1:
-        raise ValueError("x: rows need at least one element")
+    if stream is not None:
+        with _as_current(stream):
+            return quantize_rows(x)
+    code = _DTYPE_CODE.get(x.dtype)
+    if code is None or not x.is_cuda or x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x: expected a float32, float16 or bfloat16 CUDA tensor with at least one column")
     _ensure_ctx(x)
-    cols = int(x.shape[-1])
-    rows, ld = _rows_view(x, cols, "x")
-
-    def call(s):
-        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        scale = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        if lib().fastnn_b200_quantize_rows(_DTYPE_CODE[x.dtype], _ptr(x), ld, _ptr(q), _ptr(scale), rows, cols, s) != 0:
-            raise CudaError("CUDA quantize_rows failed")
-        return q, scale
-    return _on_stream(stream, call)
+    cols = x.shape[-1]
+    ld = _row_stride(x, cols, "x")
+    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
+    scale = x.new_empty(x.shape[:-1], dtype=torch.float32)
+    if lib().fastnn_b200_quantize_rows(code, x.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), x.numel() // cols, cols,
+                                       _raw_stream(x)) != 0:
+        raise CudaError("CUDA quantize_rows failed")
+    return q, scale
 
 
-def _int8_shapes(xq, x_scale, weights, act, out_dtype):
-    if not xq.is_cuda or xq.dtype != torch.int8 or not xq.is_contiguous() or xq.dim() < 1:
+def _int8_shapes(xq, x_scale, wq, act, out_dtype):
+    if xq.dtype != torch.int8 or not xq.is_cuda or xq.dim() < 1 or not xq.is_contiguous():
         raise ValueError("xq: expected a contiguous int8 CUDA tensor")
     if act not in _GATE_ACTS:
         raise ValueError("act must be ACT_NONE, ACT_RELU, ACT_GELU or ACT_SILU")
-    if out_dtype not in _DTYPE_CODE:
+    code = _DTYPE_CODE.get(out_dtype)
+    if code is None:
         raise ValueError("out_dtype must be float32, float16 or bfloat16")
-    wq = weights[0][1]
-    if wq.dim() != 2 or wq.shape[0] < 1 or wq.shape[1] < 1:
+    if wq.dim() != 2 or wq.numel() == 0:
         raise ValueError("weights must be [out_features, in_features], neither of them 0")
-    n, k = int(wq.shape[0]), int(wq.shape[1])
-    if int(xq.shape[-1]) != k:
+    n, k = wq.shape
+    if xq.shape[-1] != k:
         raise ValueError(f"Expected input features {k}")
     if k > 131071:
         raise ValueError("in_features above 131071 could overflow the 32-bit sums")
-    _check_like(x_scale, "x_scale", torch.float32, xq.device, tuple(xq.shape[:-1]))
-    for name, w, sc in weights:
-        _check_like(w, name, torch.int8, xq.device, (n, k))
-        _check_like(sc, name + " scale", torch.float32, xq.device, (n,))
+    _check_like(x_scale, "x_scale", torch.float32, xq.device, xq.shape[:-1])
     _ensure_ctx(xq)
-    return xq.numel() // k, k, n
+    return code, xq.numel() // k, k, n
+
+
+def _check_int8_weight(name, w, scale, device, n, k):
+    _check_like(w, name, torch.int8, device, (n, k))
+    _check_like(scale, name + " scale", torch.float32, device, (n,))
+
+
+def _int8_workspace(rows, k, n, gated, bits, device):
+    """(tensor to keep, pointer, bytes); rows of a multiple of 16 bytes on such bases need none."""
+    if not (bits | k) & 15:
+        return None, 0, 0
+    nbytes = lib().fastnn_b200_int8_workspace(rows, k, n, gated, 1)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr(), nbytes
 
 
 def int8_linear_forward(xq, x_scale, wq, w_scale, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None,
                         stream=None):
     """y = act(x_scale[t] * w_scale[o] * (xq . wq^T) + bias) for xq [.., in] and wq [out, in] as quantize_rows
     makes them; bias [out] float32.  The integer sums are exact; y [.., out] has ``out_dtype``."""
-    rows, k, n = _int8_shapes(xq, x_scale, (("wq", wq, w_scale),), act, out_dtype)
+    if stream is not None:
+        with _as_current(stream):
+            return int8_linear_forward(xq, x_scale, wq, w_scale, bias, act, out_dtype, out)
+    code, rows, k, n = _int8_shapes(xq, x_scale, wq, act, out_dtype)
+    _check_int8_weight("wq", wq, w_scale, xq.device, n, k)
     if bias is not None:
         _check_like(bias, "bias", torch.float32, xq.device, (n,))
-    unaligned = _unaligned(1, (xq, 0), (wq, 0))
-
-    def call(s):
-        y = _new_out(tuple(xq.shape[:-1]) + (n,), out_dtype, xq.device, out)
-        nbytes = lib().fastnn_b200_int8_workspace(rows, k, n, 0, unaligned)
-        ws = _workspace(nbytes, xq.device)
-        if lib().fastnn_b200_int8_linear_forward(_ptr(xq), _ptr(x_scale), _ptr(wq), _ptr(w_scale), _ptr(bias),
-                                                 _ptr(y), _DTYPE_CODE[out_dtype], rows, k, n, act, _ptr(ws), nbytes,
-                                                 s) != 0:
-            raise CudaError("CUDA int8_linear_forward failed")
-        return y
-    return _on_stream(stream, call)
+    px, pw = xq.data_ptr(), wq.data_ptr()
+    y = _new_out(xq.shape[:-1] + (n,), out_dtype, xq, out)
+    ws, pws, nbytes = _int8_workspace(rows, k, n, 0, px | pw, xq.device)
+    if lib().fastnn_b200_int8_linear_forward(px, x_scale.data_ptr(), pw, w_scale.data_ptr(),
+                                             0 if bias is None else bias.data_ptr(), y.data_ptr(), code, rows, k, n, act,
+                                             pws, nbytes, _raw_stream(xq)) != 0:
+        raise CudaError("CUDA int8_linear_forward failed")
+    return y
 
 
 def int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act=ACT_SILU, out_dtype=torch.float32,
                        out=None, stream=None):
     """h = act(x_scale[t] * gate_scale[o] * (xq . Wg^T)) * (x_scale[t] * up_scale[o] * (xq . Wu^T)), the first
     half of a gated block in 8-bit integers, in one launch; xq [.., in], weights [out, in], h [.., out]."""
-    rows, k, n = _int8_shapes(xq, x_scale, (("wq_gate", wq_gate, gate_scale), ("wq_up", wq_up, up_scale)), act,
-                              out_dtype)
-    unaligned = _unaligned(1, (xq, 0), (wq_gate, 0), (wq_up, 0))
-
-    def call(s):
-        h = _new_out(tuple(xq.shape[:-1]) + (n,), out_dtype, xq.device, out)
-        nbytes = lib().fastnn_b200_int8_workspace(rows, k, n, 1, unaligned)
-        ws = _workspace(nbytes, xq.device)
-        if lib().fastnn_b200_int8_gated_forward(_ptr(xq), _ptr(x_scale), _ptr(wq_gate), _ptr(gate_scale),
-                                                _ptr(wq_up), _ptr(up_scale), _ptr(h), _DTYPE_CODE[out_dtype], rows,
-                                                k, n, act, _ptr(ws), nbytes, s) != 0:
-            raise CudaError("CUDA int8_gated_forward failed")
-        return h
-    return _on_stream(stream, call)
+    if stream is not None:
+        with _as_current(stream):
+            return int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act, out_dtype, out)
+    code, rows, k, n = _int8_shapes(xq, x_scale, wq_gate, act, out_dtype)
+    _check_int8_weight("wq_gate", wq_gate, gate_scale, xq.device, n, k)
+    _check_int8_weight("wq_up", wq_up, up_scale, xq.device, n, k)
+    px, pg, pu = xq.data_ptr(), wq_gate.data_ptr(), wq_up.data_ptr()
+    h = _new_out(xq.shape[:-1] + (n,), out_dtype, xq, out)
+    ws, pws, nbytes = _int8_workspace(rows, k, n, 1, px | pg | pu, xq.device)
+    if lib().fastnn_b200_int8_gated_forward(px, x_scale.data_ptr(), pg, gate_scale.data_ptr(), pu, up_scale.data_ptr(),
+                                            h.data_ptr(), code, rows, k, n, act, pws, nbytes, _raw_stream(xq)) != 0:
+        raise CudaError("CUDA int8_gated_forward failed")
+    return h
 
 
 def gemm_ex(layout, a_ptr, b_ptr, c_ptr, m, n, k, batch, lda, ldb, ldc, sa, sb, sc,
