@@ -38,37 +38,50 @@ enum : int {
 constexpr int kActSilu = 5;
 
 constexpr int kNarrowEpiWarps = 8;
-constexpr int kNarrowThreads = 64 + 32 * kNarrowEpiWarps;
+constexpr int kNarrowMmaWarpB = 2 + kNarrowEpiWarps; // second MMA-issuing warp (wide tiles)
+constexpr int kNarrowThreads = 32 * (kNarrowMmaWarpB + 1);
 constexpr int kNarrowMaxProblems = 4;
 constexpr int kNarrowMaxStages = 8;
-constexpr int kNarrowTile = 4096;                    // one staging tile: 32 rows x 128 bytes
 constexpr int kNarrowABytes = 128 * 128;             // 128 rows x 128 bytes of K
+constexpr int kNarrowBarBytes = 512;
+// Staging tiles: 32 rows x 32 columns of the output type, rows of 64 (16-bit) or 128 bytes in the
+// swizzle of that span.
+template <typename T>
+constexpr int kTileBytes = 32 * 32 * static_cast<int>(sizeof(T));
+// Staging bytes of one epilogue warp.  Two tiles in turn, of which one is being stored while the next is
+// filled; a gradient epilogue holds sets of (gate, up, h) tiles instead, two of 16 bits or one of 32.
+// The FP32 partial sums of a K split need 4 KiB of either.
+template <int kEpi, typename T>
+constexpr int kStagingWarp = kEpi == kEpiGatedGrad ? 12288 : 4096;
 
 struct NarrowProblem {
   CUtensorMap a[2], b[2];      // [1]: second K range (C = A0.B0 + A1.B1), or the up weight of a gated product
   CUtensorMap out[3];
-  void* out_ptr[3];            // the same outputs for stores TMA cannot make; null: not wanted
+  CUtensorMap aux[2];          // kEpiGatedGrad: the saved gate and up projections
+  void* out_ptr[3];            // the outputs for stores TMA cannot make; null: not wanted
   long long out_ld[3];         // their row strides in elements
-  const void* gate;            // saved projections of kEpiGatedGrad, row stride aux_ld elements
-  const void* up;
-  long long aux_ld;
+  int tma_out[3];              // outputs are TMA-addressable
   int m, n;                    // n: columns of ONE output
   int tiles_m, tiles_n;
   int num_kb, num_kb1;         // 128-byte k-blocks in all, and those of the first operand pair
   int split_k, kb_per_split;   // split_k > 1: partial sums, FP32, one [m, n] block per slice in out[0]
   int first_unit;
   int a_mn, b_mn;              // operand stored with M (N) contiguous
-  int tma_out[3];              // outputs are TMA-addressable
 };
 
+template <int kProblems>
 struct NarrowParams {
-  NarrowProblem pr[kNarrowMaxProblems];
-  int count, total_units, block_n, num_stages, group_m;
+  NarrowProblem pr[kProblems];
+  int count, total_units;
+  int groups;                  // 256-column MMA groups of a tile: 2 for wide tiles
+  int mma_n;                   // columns of one group's MMA; a tile has groups * mma_n
+  int num_stages, group_m;
   int act, is_bf16;
   const float* row_scale;
   const float* col_scale;
   const float* col_scale2;
   const float* bias;
+  int vec_scale;               // the column vectors are 16-byte aligned
   unsigned int* status;
   long long spin_budget;
 };
@@ -179,30 +192,67 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// 32 consecutive columns of this lane's row into a staging tile (32 rows x 128 bytes, 16-byte unit j
-// of row r at unit j ^ (r & 7)).  16-bit outputs fill the lower (half = 0) or upper half of the row.
+// Byte offset of 16-byte unit j of row r in a staging tile: rows of 64 bytes in the 64-byte swizzle
+// (unit j at j ^ ((r >> 1) & 3)), rows of 128 in the 128-byte one (j ^ (r & 7)).
 template <typename T>
-__device__ __forceinline__ void stage_put(uint8_t* tile, int lane, int half, const float (&v)[32]) {
-  uint8_t* row = tile + lane * 128;
+__device__ __forceinline__ uint32_t tile_unit(int r, int j) {
+  if constexpr (sizeof(T) == 4) return static_cast<uint32_t>(r * 128 + ((j ^ (r & 7)) << 4));
+  else return static_cast<uint32_t>(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+}
+
+// This lane's row, 32 columns, to and from a staging tile.
+template <typename T>
+__device__ __forceinline__ void tile_put(uint8_t* tile, int lane, const float (&v)[32]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<float4*>(row + ((j ^ (lane & 7)) << 4)) =
+      *reinterpret_cast<float4*>(tile + tile_unit<T>(lane, j)) =
           make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(row + (((half * 4 + j) ^ (lane & 7)) << 4)) =
+      *reinterpret_cast<uint4*>(tile + tile_unit<T>(lane, j)) =
           make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
                      pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
   }
 }
+// 8 columns of it: the j-th eighth (32-bit types: two units) or unit j
+template <typename T>
+__device__ __forceinline__ void tile_get8(const uint8_t* tile, int lane, int j, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float4 f = *reinterpret_cast<const float4*>(tile + tile_unit<T>(lane, 2 * j + i));
+      v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
+    }
+  } else {
+    const uint4 w = *reinterpret_cast<const uint4*>(tile + tile_unit<T>(lane, j));
+    const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2<T>(q[i]);
+      v[2 * i] = f.x; v[2 * i + 1] = f.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void tile_put8(uint8_t* tile, int lane, int j, const float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<float4*>(tile + tile_unit<T>(lane, 2 * j + i)) =
+          make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+  } else {
+    *reinterpret_cast<uint4*>(tile + tile_unit<T>(lane, j)) =
+        make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
+  }
+}
 
-// The staging tile to output rows [m0, m0 + 32), columns from col0: one TMA store, which clips at the
+// A staging tile to output rows [m0, m0 + 32), columns from col0: one TMA store, which clips at the
 // matrix's edges, or row by row (row strides that are no multiple of 16 bytes, unaligned bases).
 template <typename T>
-__device__ __forceinline__ void stage_flush(const CUtensorMap* map, void* out, long long ld, int tma, uint8_t* tile,
-                                            uint32_t tile_addr, int m0, int col0, int z, int m, int n, int lane) {
+__device__ __forceinline__ void tile_flush(const CUtensorMap* map, void* out, long long ld, int tma, uint8_t* tile,
+                                           uint32_t tile_addr, int m0, int col0, int z, int m, int n, int lane) {
   if (tma) {
     ptx::fence_proxy_async_smem();
     __syncwarp();
@@ -213,43 +263,12 @@ __device__ __forceinline__ void stage_flush(const CUtensorMap* map, void* out, l
   } else {
     __syncwarp();
     const int rows = min(32, m - m0);
-    for (int r = 0; r < rows; ++r) {
-      const uint32_t w = *reinterpret_cast<const uint32_t*>(tile + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
-                                                            ((lane & 3) << 2));
-      T* dst = static_cast<T*>(out) + (static_cast<long long>(z) * m + m0 + r) * ld + col0;
-      if constexpr (sizeof(T) == 4) {
-        if (col0 + lane < n) reinterpret_cast<uint32_t*>(dst)[lane] = w;
-      } else {
-        uint16_t* d16 = reinterpret_cast<uint16_t*>(dst);
-        if (col0 + 2 * lane < n) d16[2 * lane] = static_cast<uint16_t>(w & 0xffffu);
-        if (col0 + 2 * lane + 1 < n) d16[2 * lane + 1] = static_cast<uint16_t>(w >> 16);
-      }
-    }
+    T* dst = static_cast<T*>(out) + static_cast<long long>(m0) * ld + col0 + lane;
+    constexpr int kPer = 16 / static_cast<int>(sizeof(T));
+    if (col0 + lane < n)
+      for (int r = 0; r < rows; ++r)
+        dst[r * ld] = *reinterpret_cast<const T*>(tile + tile_unit<T>(r, lane / kPer) + (lane % kPer) * sizeof(T));
     __syncwarp();
-  }
-}
-
-// 32 columns of this lane's row of a saved projection (16-byte aligned rows; zero outside)
-template <typename T>
-__device__ __forceinline__ void load_row32(const void* base, long long ld, int row, int col0, int m, int n,
-                                           float (&v)[32]) {
-  constexpr int kPer = 16 / sizeof(T);
-  const T* src = static_cast<const T*>(base) + static_cast<long long>(row) * ld + col0;
-#pragma unroll
-  for (int j = 0; j < 32 / kPer; ++j) {
-    uint4 w = make_uint4(0, 0, 0, 0);
-    if (row < m && col0 + j * kPer < n) w = __ldg(reinterpret_cast<const uint4*>(src + j * kPer));
-    if constexpr (sizeof(T) == 4) {
-      v[4 * j] = __uint_as_float(w.x); v[4 * j + 1] = __uint_as_float(w.y);
-      v[4 * j + 2] = __uint_as_float(w.z); v[4 * j + 3] = __uint_as_float(w.w);
-    } else {
-      const uint32_t q[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float2 f = unpack2<T>(q[i]);
-        v[8 * j + 2 * i] = f.x; v[8 * j + 2 * i + 1] = f.y;
-      }
-    }
   }
 }
 
@@ -285,10 +304,12 @@ __device__ __forceinline__ bool narrow_wait(uint32_t bar, uint32_t parity, volat
 struct NarrowUnit {
   int pr, s, mt, nt, kb0, kb1;
 };
-__device__ __forceinline__ NarrowUnit narrow_unit(const NarrowParams& p, int u) {
+template <int kProblems>
+__device__ __forceinline__ NarrowUnit narrow_unit(const NarrowParams<kProblems>& p, int u) {
   NarrowUnit w;
   int i = 0;
-  while (i + 1 < p.count && u >= p.pr[i + 1].first_unit) ++i;
+  if constexpr (kProblems > 1)
+    while (i + 1 < p.count && u >= p.pr[i + 1].first_unit) ++i;
   const NarrowProblem& q = p.pr[i];
   int t = u - q.first_unit;
   w.pr = i;
@@ -306,11 +327,12 @@ __device__ __forceinline__ NarrowUnit narrow_unit(const NarrowParams& p, int u) 
   return w;
 }
 
-template <int kKind, int kEpi, typename OutT>
+template <int kKind, int kEpi, typename OutT, int kProblems>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNarrowThreads, 1)
-narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
+narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   using K = NarrowKind<kKind>;
   constexpr bool kTwoB = kEpi == kEpiGated || kEpi == kEpiScaledGated;
+  constexpr bool kGrad = kEpi == kEpiGatedGrad;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -320,10 +342,13 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
   const uint32_t rank = ptx::cluster_ctarank();
   const int cluster_id = blockIdx.x >> 1;
   const int num_clusters = gridDim.x >> 1;
-  const int half_n = p.block_n >> 1;                     // B columns this CTA loads
-  const uint32_t stage_bytes = kNarrowABytes + static_cast<uint32_t>(half_n) * 128u;
+  const int groups = p.groups;
+  const int half_n = p.mma_n >> 1;                       // B columns of one MMA group this CTA loads
+  const int block_n = groups * p.mma_n;
+  const uint32_t half_bytes = static_cast<uint32_t>(half_n) * 128u;
+  const uint32_t stage_bytes = kNarrowABytes + static_cast<uint32_t>(groups) * half_bytes;
   const uint32_t staging_base = smem_base + p.num_stages * stage_bytes;
-  const uint32_t bar_base = staging_base + kNarrowEpiWarps * kNarrowTile;
+  const uint32_t bar_base = staging_base + kNarrowEpiWarps * kStagingWarp<kEpi, OutT>;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 64u + 8u * s; };
   auto tfull_bar = [&](int a) { return bar_base + 128u + 8u * a; };
@@ -332,20 +357,25 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
   uint8_t* bar_gen = smem_gen + (bar_base - smem_base);
   volatile uint32_t* tmem_slot_gen = reinterpret_cast<volatile uint32_t*>(bar_gen + 160);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 168);
-  float* scale_gen = reinterpret_cast<float*>(bar_gen + 256);     // 96 floats per epilogue warp (8-bit kinds)
+  auto aux_bar = [&](int ew, int set) { return bar_base + 256u + 16u * ew + 8u * set; };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.num_stages; ++s) {
       ptx::mbar_init(full_bar(s), 2);          // one arrive.expect_tx from each CTA's producer
-      ptx::mbar_init(empty_bar(s), 1);
+      ptx::mbar_init(empty_bar(s), groups);    // one commit per MMA-issuing thread
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(tfull_bar(a), 1);
       ptx::mbar_init(tempty_bar(a), 2 * kNarrowEpiWarps);
     }
+    if constexpr (kGrad)
+      for (int i = 0; i < 2 * kNarrowEpiWarps; ++i) ptx::mbar_init(bar_base + 256u + 8u * i, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
+    ptx::prefetch_tensormap(&p.pr[0].a[0]);
+    ptx::prefetch_tensormap(&p.pr[0].b[kTwoB ? rank : 0]);
+    ptx::prefetch_tensormap(&p.pr[0].out[0]);
   }
   if (warp == 1) {
     ptx::tmem_alloc_2cta(tmem_slot, kTmemCols);
@@ -357,6 +387,11 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
   ptx::cluster_wait_acquire();
   ptx::tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot_gen;
+  // Launched as a programmatic dependent: everything above overlaps the end of the kernel before, whose
+  // writes are complete only from here on.  The next kernel may in turn be placed on SMs this grid leaves
+  // (never beside one of its CTAs, which take a whole SM's shared memory and tensor memory).
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
 
   if (warp == 0) {
     // ------------------------------------------------------------- producer ---
@@ -370,14 +405,14 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
         const NarrowProblem& q = p.pr[w.pr];
         const int m0 = w.mt * 256 + static_cast<int>(rank) * 128;
         // a gated tile: this CTA's columns are all gate (leader) or all up (peer) columns of the same outputs
-        const int n0 = kTwoB ? w.nt * half_n : w.nt * p.block_n + static_cast<int>(rank) * half_n;
+        const int n0 = kTwoB ? w.nt * (block_n >> 1) : w.nt * block_n + static_cast<int>(rank) * half_n;
+        const int n_step = kTwoB ? half_n : p.mma_n;     // to the next group's columns
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           ok = narrow_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, kStatusProducerTimeout);
           if (!ok) break;
           const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0);
           ptx::mbar_expect_tx_cluster(fb, stage_bytes);
           const uint32_t sa = smem_base + stage * stage_bytes;
-          const uint32_t sb = sa + kNarrowABytes;
           const bool second = kb >= q.num_kb1;
           const int k0 = (second ? kb - q.num_kb1 : kb) * K::kBlock;
           const CUtensorMap* mA = &q.a[second ? 1 : 0];
@@ -389,11 +424,15 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
             for (int c = 0; c < 128 / static_cast<int>(K::kChunkElems); ++c)
               ptx::tma_load_3d_pair(sa + c * K::kChunkBytes, mA, fb, m0 + c * K::kChunkElems, k0, 0, pol);
           }
-          if (!q.b_mn) {
-            ptx::tma_load_3d_pair(sb, mB, fb, k0, n0, 0, pol);
-          } else {
-            for (int c = 0; c < half_n / static_cast<int>(K::kChunkElems); ++c)
-              ptx::tma_load_3d_pair(sb + c * K::kChunkBytes, mB, fb, n0 + c * K::kChunkElems, k0, 0, pol);
+          for (int g = 0; g < groups; ++g) {
+            const uint32_t sb = sa + kNarrowABytes + g * half_bytes;
+            const int ng = n0 + g * n_step;
+            if (!q.b_mn) {
+              ptx::tma_load_3d_pair(sb, mB, fb, k0, ng, 0, pol);
+            } else {
+              for (int c = 0; c < half_n / static_cast<int>(K::kChunkElems); ++c)
+                ptx::tma_load_3d_pair(sb + c * K::kChunkBytes, mB, fb, ng + c * K::kChunkElems, k0, 0, pol);
+            }
           }
           if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
         }
@@ -404,29 +443,33 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
         if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
       }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------ MMA issuer (leader only) ---
-    if (lane == 0 && rank == 0) {
+  } else if (warp == 1 || warp == kNarrowMmaWarpB) {
+    // ----------------------------------------------- MMA issuers (leader only) ---
+    // One thread per MMA group.  The two accumulator slots of 256 columns hold alternate tiles of a
+    // one-group launch, or the two groups of a wide tile; either way a slot is filled again as soon as
+    // the epilogue has drained it, so a wide tile's first group starts while its second is being read.
+    const int my_group = warp == 1 ? 0 : 1;
+    if (lane == 0 && rank == 0 && my_group < groups) {
       const uint64_t stage_step = stage_bytes >> 4;
       const uint32_t bar0 = ptx::mapa_shared(bar_base, 0);
       const uint32_t bar1 = ptx::mapa_shared(bar_base, 1);
       int stage = 0;
       uint32_t phase = 0;
-      int acc = 0;
-      uint32_t acc_phase = 0;
+      int slot = my_group;
+      uint32_t slot_phase = 0;
       bool ok = true;
       for (int u = cluster_id; u < p.total_units && ok; u += num_clusters) {
         const NarrowUnit w = narrow_unit(p, u);
         const NarrowProblem& q = p.pr[w.pr];
-        const uint32_t idesc = ptx::idesc_narrow<kKind>(256, p.block_n, q.a_mn, q.b_mn, p.is_bf16);
+        const uint32_t idesc = ptx::idesc_narrow<kKind>(256, p.mma_n, q.a_mn, q.b_mn, p.is_bf16);
         const uint64_t a_desc0 = narrow_desc<kKind>(smem_base, q.a_mn);
-        const uint64_t b_desc0 = narrow_desc<kKind>(smem_base + kNarrowABytes, q.b_mn);
+        const uint64_t b_desc0 = narrow_desc<kKind>(smem_base + kNarrowABytes + my_group * half_bytes, q.b_mn);
         const uint64_t a_step = (q.a_mn ? K::kMnStep : 32u) >> 4;
         const uint64_t b_step = (q.b_mn ? K::kMnStep : 32u) >> 4;
-        ok = narrow_wait(tempty_bar(acc), acc_phase ^ 1u, abort_flag, p, kStatusMmaTmemTimeout);
+        ok = narrow_wait(tempty_bar(slot), slot_phase ^ 1u, abort_flag, p, kStatusMmaTmemTimeout);
         if (!ok) break;
         ptx::tc_fence_after_sync();
-        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(acc * kMaxBlockN);
+        const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(slot * kMaxBlockN);
         uint32_t accumulate = 0u;
         for (int kb = w.kb0; kb < w.kb1; ++kb) {
           ok = narrow_wait(full_bar(stage), phase, abort_flag, p, kStatusMmaTimeout);
@@ -443,188 +486,271 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
           if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        ptx::mma_commit_2cta(bar0 + 128u + 8u * acc);       // accumulator full, both CTAs
-        ptx::mma_commit_2cta(bar1 + 128u + 8u * acc);
-        if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
+        ptx::mma_commit_2cta(bar0 + 128u + 8u * slot);      // accumulator full, both CTAs
+        ptx::mma_commit_2cta(bar1 + 128u + 8u * slot);
+        if (groups == 2) slot_phase ^= 1u;
+        else if (++slot == 2) { slot = 0; slot_phase ^= 1u; }
       }
     }
   } else {
     // -------------------------------------------------------------- epilogue ---
-    // Two warps per TMEM lane quadrant take alternate chunks of the tile; a chunk is what fills a
-    // staging tile, 128 bytes of a row: 64 columns of 16 bits, 32 of 32.
+    // Two warps per TMEM lane quadrant take alternate 32-column chunks of a slot.
     const int ew = warp - 2;
     const int q4 = warp & 3;
     const int group = ew >> 2;
-    const uint32_t tile_addr = staging_base + ew * kNarrowTile;
-    uint8_t* tile = smem_gen + (tile_addr - smem_base);
-    float* scales = scale_gen + ew * 96;
-    int acc = 0;
-    uint32_t acc_phase = 0;
+    const uint32_t my_addr = staging_base + ew * kStagingWarp<kEpi, OutT>;
+    uint8_t* my_gen = smem_gen + (my_addr - smem_base);
+    constexpr int kTile = kTileBytes<OutT>;
+    constexpr int kBufs = kStagingWarp<kEpi, OutT> / kTile < 2 ? 1 : 2;
+    int buf = 0;
+    int slot = 0;
+    uint32_t slot_phase = 0;
     bool ok = true;
+
+    // kGrad: the (gate, up) tiles of the next chunk are fetched while this one is computed
+    constexpr int kSets = kGrad ? kStagingWarp<kEpi, OutT> / (3 * kTile) : 1;
+    int set = 0;
+    uint32_t set_phase = 0;                                  // a bit for each set
+    bool fetched = false;                                    // the current set's tiles are on their way
+    auto set_addr = [&](int s) { return my_addr + s * 3 * kTile; };
+    auto fetch_aux = [&](const NarrowUnit& w, int c, int s) {          // lane 0
+      if constexpr (kGrad) {
+        const NarrowProblem& q = p.pr[w.pr];
+        const int m0 = w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32;
+        const int col0 = w.nt * block_n + c * 32;
+        const uint32_t bar = aux_bar(ew, s);
+        ptx::mbar_expect_tx(bar, 2 * kTile);
+        ptx::tma_load_3d(set_addr(s), &q.aux[0], bar, col0, m0, 0);
+        ptx::tma_load_3d(set_addr(s) + kTile, &q.aux[1], bar, col0, m0, 0);
+      }
+    };
+    // whether chunk c of unit u exists for this warp (its rows and columns reach into the matrix)
+    auto live = [&](const NarrowUnit& w, int c) {
+      const NarrowProblem& q = p.pr[w.pr];
+      return w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32 < q.m && w.nt * block_n + c * 32 < q.n;
+    };
+    if constexpr (kGrad) {
+      const NarrowUnit w = narrow_unit(p, cluster_id);       // the grid has no more pairs than units
+      fetched = live(w, group);
+      if (fetched && lane == 0) fetch_aux(w, group, 0);
+    }
+
     for (int u = cluster_id; u < p.total_units && ok; u += num_clusters) {
       const NarrowUnit w = narrow_unit(p, u);
       const NarrowProblem& q = p.pr[w.pr];
       const int m0 = w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32;
       const int row = m0 + lane;
       const bool raw = q.split_k > 1;
-      ok = narrow_wait(tfull_bar(acc), acc_phase, abort_flag, p, kStatusEpilogueTimeout);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-      ptx::tc_fence_after_sync();
-      const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) +
-                             static_cast<uint32_t>(acc * kMaxBlockN);
-      auto load32 = [&](int col, float (&v)[32]) {           // 32 accumulator columns as floats
-        uint32_t r[32];
-        ptx::tmem_ld_32x32(taddr + col, r);
-        ptx::tmem_ld_wait();
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-          v[j] = kKind == kKindI8 ? static_cast<float>(static_cast<int>(r[j])) : __uint_as_float(r[j]);
-      };
-      auto tile_free = [&]() {                               // the staging tile may be overwritten
-        if (lane == 0) ptx::tma_store_wait_read<0>();
-        __syncwarp();
-      };
       const bool rows_live = m0 < q.m;                       // warp-uniform
-      if (rows_live) {
-      if constexpr (kEpi == kEpiStore) {
-        const int n0 = w.nt * p.block_n;
-        if (raw) {                                           // FP32 partial sums of one K slice
-          for (int c = group; c < p.block_n / 32; c += 2) {
-            const int col0 = n0 + c * 32;
-            if (col0 >= q.n) break;
-            float v[32];
-            load32(c * 32, v);
-            tile_free();
-            stage_put<float>(tile, lane, 0, v);
-            stage_flush<float>(&q.out[0], q.out_ptr[0], q.out_ld[0], true, tile, tile_addr, m0, col0, w.s, q.m, q.n, lane);
-          }
-        } else {
-          constexpr int kCols = 128 / sizeof(OutT);
-          for (int c = group; c < p.block_n / kCols; c += 2) {
-            const int col0 = n0 + c * kCols;
-            if (col0 >= q.n) break;
-            tile_free();
+      for (int g = 0; g < groups && ok; ++g) {
+        ok = narrow_wait(tfull_bar(slot), slot_phase, abort_flag, p, kStatusEpilogueTimeout);
+        ok = __all_sync(0xffffffffu, ok);
+        if (!ok) break;
+        ptx::tc_fence_after_sync();
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) +
+                               static_cast<uint32_t>(slot * kMaxBlockN);
+        auto load32 = [&](int col, uint32_t (&r)[32]) { ptx::tmem_ld_32x32(taddr + col, r); };
+        auto value = [&](uint32_t r) {
+          return kKind == kKindI8 ? static_cast<float>(static_cast<int>(r)) : __uint_as_float(r);
+        };
+        auto next_tile = [&]() {                             // a staging tile that may be overwritten
+          if constexpr (kBufs == 2) buf ^= 1;
+          if (lane == 0) ptx::tma_store_wait_read<kBufs - 1>();
+          __syncwarp();
+        };
+        if (rows_live) {
+          if constexpr (kEpi == kEpiStore) {
+            const int n0 = w.nt * block_n + g * p.mma_n;
+            if (raw) {                                       // FP32 partial sums of one K slice
+              for (int c = group; c < p.mma_n / 32; c += 2) {
+                const int col0 = n0 + c * 32;
+                if (col0 >= q.n) break;
+                uint32_t r[32];
+                load32(c * 32, r);
+                if (lane == 0) ptx::tma_store_wait_read<0>();
+                __syncwarp();
+                ptx::tmem_ld_wait();
+                float v[32];
 #pragma unroll
-            for (int h = 0; h < kCols / 32; ++h) {
-              float v[32];
-              load32(c * kCols + h * 32, v);
-              stage_put<OutT>(tile, lane, h, v);
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                tile_put<float>(my_gen, lane, v);
+                tile_flush<float>(&q.out[0], nullptr, 0, 1, my_gen, my_addr, m0, col0, w.s, q.m, q.n, lane);
+              }
+            } else {
+              for (int c = group; c < p.mma_n / 32; c += 2) {
+                const int col0 = n0 + c * 32;
+                if (col0 >= q.n) break;
+                uint32_t r[32];
+                load32(c * 32, r);
+                next_tile();
+                ptx::tmem_ld_wait();
+                float v[32];
+#pragma unroll
+                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+                tile_put<OutT>(my_gen + buf * kTile, lane, v);
+                tile_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], my_gen + buf * kTile,
+                                 my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+              }
             }
-            stage_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], tile, tile_addr, m0, col0, 0, q.m, q.n, lane);
-          }
-        }
-      } else if constexpr (kEpi == kEpiGated) {
-        constexpr int kCols = 128 / sizeof(OutT);
-        const int n0 = w.nt * half_n;
-        for (int c = group; c < half_n / kCols; c += 2) {
-          const int col0 = n0 + c * kCols;
-          if (col0 >= q.n) break;
-          tile_free();
+          } else if constexpr (kEpi == kEpiGated) {
+            const int n0 = w.nt * (block_n >> 1) + g * half_n;
+            const bool save = q.out_ptr[1] != nullptr;
+            for (int c = group; c < half_n / 32; c += 2) {
+              const int col0 = n0 + c * 32;
+              if (col0 >= q.n) break;
+              uint32_t rg[32], ru[32];
+              load32(c * 32, rg);
+              load32(half_n + c * 32, ru);
+              next_tile();
+              ptx::tmem_ld_wait();
+              float gv[32], v[32];
 #pragma unroll
-          for (int h = 0; h < kCols / 32; ++h) {
-            float g[32], v[32];
-            load32(c * kCols + h * 32, g);
-            load32(half_n + c * kCols + h * 32, v);
-            for_act(p.act, [&](auto tag) {
-                constexpr int kAct = decltype(tag)::value;
-#pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] *= gate_act<kAct>(g[j]);
-            });
-            stage_put<OutT>(tile, lane, h, v);
-          }
-          stage_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], tile, tile_addr, m0, col0, 0, q.m, q.n, lane);
-          // the projections themselves, for the backward pass: read again, so that no thread holds three rows
-          for (int i = 1; i <= 2; ++i) {
-            if (q.out_ptr[i] == nullptr) continue;
-            tile_free();
-#pragma unroll
-            for (int h = 0; h < kCols / 32; ++h) {
-              float v[32];
-              load32((i - 1) * half_n + c * kCols + h * 32, v);
-              stage_put<OutT>(tile, lane, h, v);
-            }
-            stage_flush<OutT>(&q.out[i], q.out_ptr[i], q.out_ld[i], q.tma_out[i], tile, tile_addr, m0, col0, 0, q.m, q.n, lane);
-          }
-        }
-      } else if constexpr (kEpi == kEpiGatedGrad) {
-        constexpr int kCols = 128 / sizeof(OutT);
-        const int n0 = w.nt * p.block_n;
-        for (int c = group; c < p.block_n / kCols; c += 2) {
-          const int col0 = n0 + c * kCols;
-          if (col0 >= q.n) break;
-#pragma unroll 1
-          for (int i = 0; i < 3; ++i) {
-            tile_free();
-#pragma unroll 1
-            for (int h = 0; h < kCols / 32; ++h) {
-              float dh[32], g[32], up[32];
-              load_row32<OutT>(q.gate, q.aux_ld, row, col0 + h * 32, q.m, q.n, g);
-              if (i != 1) load_row32<OutT>(q.up, q.aux_ld, row, col0 + h * 32, q.m, q.n, up);
-              if (i != 2) load32(c * kCols + h * 32, dh);
+              for (int j = 0; j < 32; ++j) { gv[j] = __uint_as_float(rg[j]); v[j] = __uint_as_float(ru[j]); }
+              if (save) {                                    // the projections themselves, for the backward pass
+                tile_put<OutT>(my_gen + buf * kTile, lane, gv);
+                tile_flush<OutT>(&q.out[1], q.out_ptr[1], q.out_ld[1], q.tma_out[1], my_gen + buf * kTile,
+                                 my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+                next_tile();
+                tile_put<OutT>(my_gen + buf * kTile, lane, v);
+                tile_flush<OutT>(&q.out[2], q.out_ptr[2], q.out_ld[2], q.tma_out[2], my_gen + buf * kTile,
+                                 my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+                next_tile();
+              }
               for_act(p.act, [&](auto tag) {
                 constexpr int kAct = decltype(tag)::value;
 #pragma unroll
-                for (int j = 0; j < 32; ++j) {
-                  float a, da;
-                  gate_act_grad<kAct>(g[j], a, da);
-                  dh[j] = i == 0 ? dh[j] * up[j] * da : (i == 1 ? dh[j] * a : a * up[j]);
+                for (int j = 0; j < 32; ++j) v[j] *= gate_act<kAct>(gv[j]);
+              });
+              tile_put<OutT>(my_gen + buf * kTile, lane, v);
+              tile_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], my_gen + buf * kTile,
+                               my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+            }
+          } else if constexpr (kGrad) {
+            // dgate and dup take the places of gate and up in the set's tiles (a lane reads and writes
+            // its own row), h a third tile; all three rows are addressable by construction
+            const int n0 = w.nt * block_n;
+            for (int c = group; c < block_n / 32; c += 2) {
+              const int col0 = n0 + c * 32;
+              if (col0 >= q.n) break;
+              uint32_t r[32];
+              load32(c * 32, r);
+              uint8_t* tiles = my_gen + set * 3 * kTile;
+              NarrowUnit wn = w;                             // the chunk this warp comes to next
+              int cn = c + 2;
+              bool more = cn * 32 < block_n && live(wn, cn);
+              if (!more && u + num_clusters < p.total_units) {
+                wn = narrow_unit(p, u + num_clusters);
+                cn = group;
+                more = live(wn, cn);
+              }
+              if (lane == 0) {
+                // every store so far has read its tiles: these may be filled again
+                if (!fetched || kSets == 2) ptx::tma_store_wait_read<0>();
+                if (!fetched) fetch_aux(w, c, set);
+                if (kSets == 2 && more) fetch_aux(wn, cn, set ^ 1);
+              }
+              __syncwarp();
+              ok = narrow_wait(aux_bar(ew, set), (set_phase >> set) & 1u, abort_flag, p, kStatusEpilogueTimeout);
+              ok = __all_sync(0xffffffffu, ok);
+              if (!ok) break;
+              set_phase ^= 1u << set;
+              ptx::tmem_ld_wait();
+              for_act(p.act, [&](auto tag) {
+                constexpr int kAct = decltype(tag)::value;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                  float gv[8], uv[8], hv[8];
+                  tile_get8<OutT>(tiles, lane, j, gv);
+                  tile_get8<OutT>(tiles + kTile, lane, j, uv);
+#pragma unroll
+                  for (int i = 0; i < 8; ++i) {
+                    float a, da;
+                    gate_act_grad<kAct>(gv[i], a, da);
+                    const float dh = __uint_as_float(r[8 * j + i]);
+                    hv[i] = a * uv[i];
+                    gv[i] = dh * uv[i] * da;
+                    uv[i] = dh * a;
+                  }
+                  tile_put8<OutT>(tiles, lane, j, gv);
+                  tile_put8<OutT>(tiles + kTile, lane, j, uv);
+                  tile_put8<OutT>(tiles + 2 * kTile, lane, j, hv);
                 }
               });
-              stage_put<OutT>(tile, lane, h, dh);
+              ptx::fence_proxy_async_smem();
+              __syncwarp();
+              if (lane == 0) {
+                const uint32_t ta = set_addr(set);
+                ptx::tma_store_3d(&q.out[0], ta, col0, m0, 0);
+                ptx::tma_store_3d(&q.out[1], ta + kTile, col0, m0, 0);
+                ptx::tma_store_3d(&q.out[2], ta + 2 * kTile, col0, m0, 0);
+                ptx::tma_store_commit();
+                if (kSets == 1 && more) {
+                  ptx::tma_store_wait_read<0>();
+                  fetch_aux(wn, cn, 0);
+                }
+              }
+              fetched = more;
+              if constexpr (kSets == 2) set ^= 1;
             }
-            stage_flush<OutT>(&q.out[i], q.out_ptr[i], q.out_ld[i], q.tma_out[i], tile, tile_addr, m0, col0, 0, q.m, q.n, lane);
-          }
-        }
-      } else {
-        // 8-bit products: the scale of this lane's row, the scales (and bias) of 32 columns through a
-        // few bytes of shared memory, read back as broadcasts
-        constexpr int kCols = 128 / sizeof(OutT);
-        constexpr bool kGated = kEpi == kEpiScaledGated;
-        const float rs = row < q.m ? __ldg(p.row_scale + row) : 0.0f;
-        const int width = kGated ? half_n : p.block_n;
-        const int n0 = w.nt * width;
-        for (int c = group; c < width / kCols; c += 2) {
-          const int col0 = n0 + c * kCols;
-          if (col0 >= q.n) break;
-          tile_free();
+          } else {
+            // 8-bit products: the scale of this lane's row, and the scales (and bias) of the 32 columns,
+            // which all lanes read from the same addresses
+            constexpr bool kGated = kEpi == kEpiScaledGated;
+            const float rs = row < q.m ? __ldg(p.row_scale + row) : 0.0f;
+            const int width = kGated ? half_n : p.mma_n;
+            const int n0 = w.nt * (kGated ? block_n >> 1 : block_n) + g * width;
+            for (int c = group; c < width / 32; c += 2) {
+              const int col0 = n0 + c * 32;
+              if (col0 >= q.n) break;
+              uint32_t r[32], ru[32];
+              load32(c * 32, r);
+              if constexpr (kGated) load32(half_n + c * 32, ru);
+              next_tile();
+              ptx::tmem_ld_wait();
+              float v[32];
+              const bool whole = p.vec_scale && col0 + 32 <= q.n;
+              auto column4 = [&](const float* src, int j) {
+                if (whole) return __ldg(reinterpret_cast<const float4*>(src + col0) + j);
+                const int k = col0 + 4 * j;
+                return make_float4(k < q.n ? __ldg(src + k) : 0.0f, k + 1 < q.n ? __ldg(src + k + 1) : 0.0f,
+                                   k + 2 < q.n ? __ldg(src + k + 2) : 0.0f, k + 3 < q.n ? __ldg(src + k + 3) : 0.0f);
+              };
 #pragma unroll
-          for (int h = 0; h < kCols / 32; ++h) {
-            const int cl = col0 + h * 32 + lane;
-            const bool in = cl < q.n;
-            scales[lane] = in ? __ldg(p.col_scale + cl) : 0.0f;
-            if constexpr (kGated) scales[32 + lane] = in ? __ldg(p.col_scale2 + cl) : 0.0f;
-            else scales[64 + lane] = (in && p.bias != nullptr) ? __ldg(p.bias + cl) : 0.0f;
-            __syncwarp();
-            float v[32];
-            load32(c * kCols + h * 32, v);
-            if constexpr (kGated) {
-              float up[32];
-              load32(half_n + c * kCols + h * 32, up);
+              for (int j = 0; j < 8; ++j) {
+                const float4 cs = column4(p.col_scale, j);
+                if constexpr (kGated) {
+                  const float4 c2 = column4(p.col_scale2, j);
+                  const float x[4] = {c2.x, c2.y, c2.z, c2.w};
+#pragma unroll
+                  for (int i = 0; i < 4; ++i)
+                    ru[4 * j + i] = __float_as_uint(value(ru[4 * j + i]) * (rs * x[i]));
+                  v[4 * j] = value(r[4 * j]) * (rs * cs.x); v[4 * j + 1] = value(r[4 * j + 1]) * (rs * cs.y);
+                  v[4 * j + 2] = value(r[4 * j + 2]) * (rs * cs.z); v[4 * j + 3] = value(r[4 * j + 3]) * (rs * cs.w);
+                } else {
+                  const float4 b = p.bias != nullptr ? column4(p.bias, j) : make_float4(0.f, 0.f, 0.f, 0.f);
+                  v[4 * j] = fmaf(value(r[4 * j]), rs * cs.x, b.x);
+                  v[4 * j + 1] = fmaf(value(r[4 * j + 1]), rs * cs.y, b.y);
+                  v[4 * j + 2] = fmaf(value(r[4 * j + 2]), rs * cs.z, b.z);
+                  v[4 * j + 3] = fmaf(value(r[4 * j + 3]), rs * cs.w, b.w);
+                }
+              }
               for_act(p.act, [&](auto tag) {
                 constexpr int kAct = decltype(tag)::value;
 #pragma unroll
                 for (int j = 0; j < 32; ++j)
-                  v[j] = gate_act<kAct>(v[j] * (rs * scales[j])) * (up[j] * (rs * scales[32 + j]));
+                  v[j] = kGated ? gate_act<kAct>(v[j]) * __uint_as_float(ru[j]) : gate_act<kAct>(v[j]);
               });
-            } else {
-              for_act(p.act, [&](auto tag) {
-                constexpr int kAct = decltype(tag)::value;
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = gate_act<kAct>(fmaf(v[j], rs * scales[j], scales[64 + j]));
-              });
+              tile_put<OutT>(my_gen + buf * kTile, lane, v);
+              tile_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], my_gen + buf * kTile,
+                               my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
             }
-            __syncwarp();
-            stage_put<OutT>(tile, lane, h, v);
           }
-          stage_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], tile, tile_addr, m0, col0, 0, q.m, q.n, lane);
         }
+        ptx::tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(tempty_bar(slot), 0));
+        if (++slot == 2) { slot = 0; slot_phase ^= 1u; }
       }
-      }
-      ptx::tc_fence_before_sync();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(ptx::mapa_shared(tempty_bar(acc), 0));
-      if (++acc == 2) { acc = 0; acc_phase ^= 1u; }
     }
     if (lane == 0) ptx::tma_store_wait_all<0>();
   }
@@ -646,10 +772,9 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams p) {
   }
 }
 
-constexpr int kNarrowTailBytes = 256 + kNarrowEpiWarps * 96 * 4;     // barriers, then the column scales
-inline size_t narrow_pair_smem_bytes(int block_n, int num_stages) {
-  return 1024 + static_cast<size_t>(num_stages) * (kNarrowABytes + block_n / 2 * 128) +
-         kNarrowEpiWarps * kNarrowTile + kNarrowTailBytes;
+// Shared memory beside the stages.
+inline size_t narrow_fixed_bytes(int epi) {
+  return 1024 + kNarrowEpiWarps * static_cast<size_t>(epi == kEpiGatedGrad ? 12288 : 4096) + kNarrowBarBytes;
 }
 
 // ------------------------------------------------------------- K-split reduction ---
@@ -667,6 +792,8 @@ struct NarrowReduceParams {
 constexpr int kReduceCols = 4;                     // columns per thread
 template <typename T>
 __global__ void __launch_bounds__(256) narrow_reduce_kernel(const __grid_constant__ NarrowReduceParams p) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
   int i = 0;
   while (i + 1 < p.count && static_cast<int>(blockIdx.x) >= p.it[i + 1].first_block) ++i;
   const NarrowReduceItem& q = p.it[i];
@@ -705,6 +832,8 @@ struct PackParams {
 };
 constexpr int kPackWords = 4 * 256;                  // destination words of one block (rows are not shared)
 __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ PackParams p) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
   int i = 0;
   while (i + 1 < p.count && static_cast<int>(blockIdx.x) >= p.it[i + 1].first_block) ++i;
   const PackItem& q = p.it[i];

@@ -28,9 +28,10 @@ bool gate_act_ok(int act) {
          act == FASTNN_B200_ACT_SILU;
 }
 
-// Tensor map of a row-major [d1, d0] matrix (x `d2` slices), 128-byte swizzle, zero outside.
+enum MapSwizzle : uint32_t { kSwz128 = 0, kSwz128Atom32 = 1, kSwz64 = 2 };
+// Tensor map of a row-major [d1, d0] matrix (x `d2` slices), zero outside.
 bool encode_narrow(CUtensorMap* map, const DType& t, const void* base, uint64_t d0, uint64_t d1, uint64_t d2,
-                   uint64_t pitch, uint64_t slice, uint32_t box0, uint32_t box1, bool atom32) {
+                   uint64_t pitch, uint64_t slice, uint32_t box0, uint32_t box1, MapSwizzle swz) {
   const EncodeTiledFn encode = g_encode.load(std::memory_order_acquire);
   if (encode == nullptr) return false;
   MapKey key;
@@ -39,7 +40,7 @@ bool encode_narrow(CUtensorMap* map, const DType& t, const void* base, uint64_t 
   key.d[0] = d0; key.d[1] = d1; key.d[2] = d2;
   key.s[0] = pitch; key.s[1] = slice;
   key.box[0] = box0; key.box[1] = box1; key.box[2] = 1;
-  key.kind = 16u + 2u * static_cast<uint32_t>(t.map) + (atom32 ? 1u : 0u);
+  key.kind = 16u + 4u * static_cast<uint32_t>(t.map) + swz;
   if (map_cache_get(key, map)) return true;
   cuuint64_t dims[3] = {d0, d1, d2};
   cuuint64_t strides[2] = {pitch, slice};
@@ -47,10 +48,32 @@ bool encode_narrow(CUtensorMap* map, const DType& t, const void* base, uint64_t 
   cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = encode(map, t.map, 3, const_cast<void*>(base), dims, strides, box, estr,
                             CU_TENSOR_MAP_INTERLEAVE_NONE,
-                            atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B,
+                            swz == kSwz64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                            : (swz == kSwz128Atom32 ? CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B : CU_TENSOR_MAP_SWIZZLE_128B),
                             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r == CUDA_SUCCESS) map_cache_put(key, *map);
   return r == CUDA_SUCCESS;
+}
+
+// A launch that may be placed while the kernel before it is finishing (the kernels wait for it before they
+// touch global memory).
+template <typename... Params, typename... Args>
+int launch_dependent(void (*kernel)(Params...), unsigned grid, unsigned block, size_t smem, cudaStream_t stream,
+                     const Args&... args) {
+  cudaLaunchConfig_t cfg;
+  std::memset(&cfg, 0, sizeof(cfg));
+  cfg.gridDim = dim3(grid, 1, 1);
+  cfg.blockDim = dim3(block, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = tunables().pdl ? 1 : 0;
+  FNN_CUDA_OK(cudaLaunchKernelEx(&cfg, kernel, args...));
+  g_launches.fetch_add(1, std::memory_order_relaxed);
+  return 0;
 }
 
 // A row-major matrix as a call gives it; `ld` in elements.
@@ -109,10 +132,7 @@ struct Packer {
   }
   int launch(cudaStream_t s) {
     if (blocks == 0) return 0;
-    fnn::pack_rows_kernel<<<blocks, 256, 0, s>>>(p);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    FNN_CUDA_OK(cudaGetLastError());
-    return 0;
+    return launch_dependent(fnn::pack_rows_kernel, static_cast<unsigned>(blocks), 256, 0, s, p);
   }
 };
 
@@ -123,8 +143,7 @@ struct NarrowTask {
   int m = 0, n = 0, k = 0, k2 = 0;
   void* out[3] = {nullptr, nullptr, nullptr};
   long long out_ld[3] = {0, 0, 0};
-  const void* gate = nullptr;
-  const void* up = nullptr;
+  const void* aux[2] = {nullptr, nullptr};     // kEpiGatedGrad: gate and up
   long long aux_ld = 0;
   // plan
   int split = 1, kb_per_split = 0, num_kb1 = 0, num_kb = 0;
@@ -135,54 +154,59 @@ struct NarrowPlan {
   int block_n;
 };
 
-// Tile width and K split of a launch.  Cost in SM clocks of the busiest CTA pair: a 128-byte k-block of
-// a 256 x block_n tile takes the tensor cores 2 * block_n clocks and its loads (16 KiB of A and
-// block_n / 2 rows of B per CTA) 1 / 64 clock a byte; a unit costs about 2000 clocks beside its k-blocks
-// (pipeline fill, the drain of its accumulator at the end of a wave), and a K split the reduction's
-// bytes and launch.  Units go round robin over the pairs, so their sums are exact.
+// Tile width and K split of a launch: the least time of the busiest CTA pair, in SM clocks.  Units go
+// round robin over the pairs, so their sums are exact; what a unit takes is a model of measured parts:
+// clocks of a 128-byte k-block by tile width (512 columns: two MMA groups over one A tile, the fewest
+// bytes an SM takes in per product; 128 and less are bound by the loads), the drain of an accumulator
+// (under the next main loop, except a wide tile's, of which a part shows), the pipeline's fill, and for a
+// K split the reduction's launch and bytes.
+inline bool epi_gated(int epi) { return epi == fnn::kEpiGated || epi == fnn::kEpiScaledGated; }
 struct PlanChoice {
   int block_n, len;          // len: k-blocks of a unit, at most
 };
-PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int clusters, bool gated, bool may_split) {
+PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int clusters, int epi, bool may_split,
+                         int want_bn, int want_split) {
   int max_kb = 1;
   for (int i = 0; i < count; ++i)
     if (t[i].num_kb > max_kb) max_kb = t[i].num_kb;
   double best = 1e300;
   int best_bn = 256, best_len = max_kb;
   // a CTA's half of an MN-major B tile is whole 128-byte chunks of N
-  int min_bn = gated ? 128 : 64;
+  int min_bn = epi_gated(epi) ? 128 : 64;
   for (int i = 0; i < count; ++i)
     if (t[i].b_mn && min_bn < 2 * kblock) min_bn = 2 * kblock;
-  for (int bn = min_bn; bn <= 256; bn *= 2) {
-    const double load = (fnn::kNarrowABytes + bn / 2 * 128) / 64.0;
-    const double per_kb = 2.0 * bn > load ? 2.0 * bn : load;
+  const int max_bn = epi == fnn::kEpiGatedGrad ? 256 : 512;
+  for (int bn = min_bn; bn <= max_bn; bn *= 2) {
+    if (want_bn >= min_bn && want_bn <= max_bn && bn != want_bn) continue;
+    const double per_kb = bn == 512 ? 1100.0 : (bn == 256 ? 620.0 : (bn == 128 ? 400.0 : 330.0));
+    const double drain = (epi == fnn::kEpiGatedGrad ? 6000.0 : 2500.0) * bn / 256.0;
     for (int parts = 1; parts <= (may_split ? 64 : 1); parts += parts < 8 ? 1 : (parts < 16 ? 2 : 8)) {
       const int len = ceil_div(max_kb, parts);                  // k-blocks of a unit, at most
       if (parts > 1 && len < 4) break;
+      if (may_split && want_split > 0 && parts != want_split) continue;
       double most = 0.0, reduce = 0.0;
-      int first = 0;
+      double unit[fnn::kNarrowMaxProblems];
+      long long units[fnn::kNarrowMaxProblems];
+      for (int i = 0; i < count; ++i) {
+        const int split = ceil_div(t[i].num_kb, len);
+        const double main = ceil_div(t[i].num_kb, split) * per_kb;
+        unit[i] = (main > drain ? main : drain) + 300.0 + (bn == 512 ? 0.3 * drain : 0.0);
+        units[i] = 1ll * ceil_div(t[i].m, 256) * ceil_div(t[i].n, epi_gated(epi) ? bn / 2 : bn) * split;
+        if (split > 1) reduce += 8.0 * split * t[i].m * t[i].n / 3400.0 / 2.0;   // written and read, mostly in L2
+      }
       // units of problem i on pair c: those u in [first, first + units) with u % clusters == c
       for (int c = 0; c < clusters; ++c) {
         double sum = 0.0;
-        first = 0;
+        long long first = 0;
         for (int i = 0; i < count; ++i) {
-          const int split = ceil_div(t[i].num_kb, len);
-          const int per = ceil_div(t[i].num_kb, split);
-          const int cols = gated ? bn / 2 : bn;
-          const long long units = 1ll * ceil_div(t[i].m, 256) * ceil_div(t[i].n, cols) * split;
-          const long long lo = (c - first % clusters + clusters) % clusters;
-          const long long mine = lo < units ? (units - lo + clusters - 1) / clusters : 0;
-          sum += mine * (per * per_kb + 2000.0);
-          first += static_cast<int>(units % clusters);
+          const long long lo = (c - first + clusters) % clusters;
+          sum += (lo < units[i] ? (units[i] - lo + clusters - 1) / clusters : 0) * unit[i];
+          first = (first + units[i]) % clusters;
         }
         if (sum > most) most = sum;
       }
-      for (int i = 0; i < count; ++i) {
-        const int split = ceil_div(t[i].num_kb, len);
-        if (split > 1) reduce += 8.0 * split * t[i].m * t[i].n / 3400.0 / 2.0;   // written and read, mostly in L2
-      }
       if (reduce > 0.0) reduce += 5000.0;
-      const double cost = most + reduce;
+      const double cost = most + drain + reduce;
       if (cost < best) { best = cost; best_bn = bn; best_len = len; }
     }
   }
@@ -191,7 +215,7 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
 
 // The choice walks some ten thousand combinations; programs repeat a handful of shapes, so answers are
 // remembered by shape.
-NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool gated, bool may_split) {
+NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, int epi, bool may_split) {
   struct Slot {
     int key[24];
     PlanChoice choice;
@@ -200,12 +224,12 @@ NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool 
   constexpr int kSlots = 512;
   static Slot memo[kSlots];
   static std::mutex memo_mutex;
-  int key[24] = {kblock, clusters, gated ? 1 : 0, may_split ? 1 : 0, count};
+  int key[24] = {kblock, clusters, epi, may_split ? 1 : 0, count, t_policy.block_n, t_policy.split_k};
   uint64_t h = 0x9E3779B97F4A7C15ull;
   for (int i = 0; i < count; ++i) {
     t[i].num_kb1 = ceil_div(t[i].k, kblock);
     t[i].num_kb = t[i].num_kb1 + (t[i].k2 > 0 ? ceil_div(t[i].k2, kblock) : 0);
-    int* q = key + 5 + 4 * i;
+    int* q = key + 7 + 4 * i;
     q[0] = t[i].m; q[1] = t[i].n; q[2] = t[i].num_kb; q[3] = t[i].b_mn ? 1 : 0;
   }
   for (int v : key) h = (h ^ static_cast<uint32_t>(v)) * 0x100000001B3ull;
@@ -214,7 +238,7 @@ NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, bool 
     std::lock_guard<std::mutex> lock(memo_mutex);
     Slot& slot = memo[(h >> 24) % kSlots];
     if (!slot.valid || std::memcmp(slot.key, key, sizeof(key)) != 0) {
-      slot.choice = choose_narrow(t, count, kblock, clusters, gated, may_split);
+      slot.choice = choose_narrow(t, count, kblock, clusters, epi, may_split, t_policy.block_n, t_policy.split_k);
       std::memcpy(slot.key, key, sizeof(key));
       slot.valid = true;
     }
@@ -236,28 +260,33 @@ void reserve_partials(Carver& ws, NarrowTask* t, int count) {
       t[i].partials = static_cast<float*>(ws.take(sizeof(float) * static_cast<size_t>(partial_ld(t[i])) * t[i].m * t[i].split));
 }
 
-typedef void (*NarrowKernel)(fnn::NarrowParams);
-// Every instantiation, for the shared-memory attribute and for dispatch: [dtype][epilogue]
-NarrowKernel pair_kernel(int kind, int epi, int out_code) {
+template <int N>
+using NarrowKernel = void (*)(fnn::NarrowParams<N>);
+// The instantiation for an operand kind, epilogue and output type; null where there is none.  Only the
+// gradients' products share a launch.
+template <int N>
+NarrowKernel<N> pair_kernel(int kind, int epi, int out_code) {
   using namespace fnn;
+  const bool bf = out_code == FASTNN_B200_BF16;
   if (kind == kKindF16) {
-    const bool bf = out_code == FASTNN_B200_BF16;
-    if (epi == kEpiStore) return bf ? &narrow_pair_kernel<kKindF16, kEpiStore, __nv_bfloat16> : &narrow_pair_kernel<kKindF16, kEpiStore, __half>;
-    if (epi == kEpiGated) return bf ? &narrow_pair_kernel<kKindF16, kEpiGated, __nv_bfloat16> : &narrow_pair_kernel<kKindF16, kEpiGated, __half>;
-    if (epi == kEpiGatedGrad) return bf ? &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __nv_bfloat16> : &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __half>;
+    if (epi == kEpiStore) return bf ? &narrow_pair_kernel<kKindF16, kEpiStore, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiStore, __half, N>;
+    if constexpr (N == 1) {
+      if (epi == kEpiGated) return bf ? &narrow_pair_kernel<kKindF16, kEpiGated, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiGated, __half, N>;
+      if (epi == kEpiGatedGrad) return bf ? &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __half, N>;
+    }
   } else if (kind == kKindTf32) {
-    if (epi == kEpiStore) return &narrow_pair_kernel<kKindTf32, kEpiStore, float>;
-    if (epi == kEpiGated) return &narrow_pair_kernel<kKindTf32, kEpiGated, float>;
-    if (epi == kEpiGatedGrad) return &narrow_pair_kernel<kKindTf32, kEpiGatedGrad, float>;
-  } else {
+    if (epi == kEpiStore) return &narrow_pair_kernel<kKindTf32, kEpiStore, float, N>;
+    if constexpr (N == 1) {
+      if (epi == kEpiGated) return &narrow_pair_kernel<kKindTf32, kEpiGated, float, N>;
+      if (epi == kEpiGatedGrad) return &narrow_pair_kernel<kKindTf32, kEpiGatedGrad, float, N>;
+    }
+  } else if constexpr (N == 1) {
     if (epi == kEpiScaled)
-      return out_code == FASTNN_B200_F32 ? &narrow_pair_kernel<kKindI8, kEpiScaled, float>
-             : (out_code == FASTNN_B200_BF16 ? &narrow_pair_kernel<kKindI8, kEpiScaled, __nv_bfloat16>
-                                             : &narrow_pair_kernel<kKindI8, kEpiScaled, __half>);
+      return out_code == FASTNN_B200_F32 ? &narrow_pair_kernel<kKindI8, kEpiScaled, float, N>
+             : (bf ? &narrow_pair_kernel<kKindI8, kEpiScaled, __nv_bfloat16, N> : &narrow_pair_kernel<kKindI8, kEpiScaled, __half, N>);
     if (epi == kEpiScaledGated)
-      return out_code == FASTNN_B200_F32 ? &narrow_pair_kernel<kKindI8, kEpiScaledGated, float>
-             : (out_code == FASTNN_B200_BF16 ? &narrow_pair_kernel<kKindI8, kEpiScaledGated, __nv_bfloat16>
-                                             : &narrow_pair_kernel<kKindI8, kEpiScaledGated, __half>);
+      return out_code == FASTNN_B200_F32 ? &narrow_pair_kernel<kKindI8, kEpiScaledGated, float, N>
+             : (bf ? &narrow_pair_kernel<kKindI8, kEpiScaledGated, __nv_bfloat16, N> : &narrow_pair_kernel<kKindI8, kEpiScaledGated, __half, N>);
   }
   return nullptr;
 }
@@ -291,8 +320,9 @@ int narrow_init() {
   for (int kind = 0; kind <= 2; ++kind)
     for (int epi = 0; epi <= 4; ++epi)
       for (int c : codes) {
-        NarrowKernel k = pair_kernel(kind, epi, c);
-        if (k != nullptr)
+        if (auto k = pair_kernel<1>(kind, epi, c))
+          FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
+        if (auto k = pair_kernel<fnn::kNarrowMaxProblems>(kind, epi, c))
           FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
         SkinnyKernel sk = skinny_kernel(kind, epi, c);
         if (sk != nullptr)
@@ -312,18 +342,20 @@ struct NarrowLaunch {
   const float* bias = nullptr;
 };
 
+template <int N>
 int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int count, const NarrowPlan& plan,
                 cudaStream_t stream) {
   using namespace fnn;
-  static thread_local NarrowParams p;
+  NarrowParams<N> p;
   std::memset(&p, 0, sizeof(p));
-  const bool gated = l.epi == kEpiGated || l.epi == kEpiScaledGated;
+  const bool gated = epi_gated(l.epi);
   const int kblock = 128 / l.in.bytes;
-  const uint32_t half_n = plan.block_n / 2;
-  DType out;
-  if (!dtype_of(l.out_code, &out)) return -1;
-  DType f32;
-  dtype_of(FASTNN_B200_F32, &f32);
+  p.groups = plan.block_n > kMaxBlockN ? 2 : 1;
+  p.mma_n = plan.block_n / p.groups;
+  const uint32_t half_n = p.mma_n / 2;
+  DType out, f32;
+  if (!dtype_of(l.out_code, &out) || !dtype_of(FASTNN_B200_F32, &f32)) return -1;
+  const MapSwizzle out_swz = out.bytes == 4 ? kSwz128 : kSwz64;
   bool ok = true;
   long long units = 0;
   for (int i = 0; i < count; ++i) {
@@ -331,27 +363,31 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
     NarrowProblem& d = p.pr[i];
     d.m = q.m; d.n = q.n;
     d.tiles_m = ceil_div(q.m, 256);
-    d.tiles_n = ceil_div(q.n, gated ? static_cast<int>(half_n) : plan.block_n);
+    d.tiles_n = ceil_div(q.n, gated ? plan.block_n / 2 : plan.block_n);
     d.num_kb = q.num_kb; d.num_kb1 = q.num_kb1;
     d.split_k = q.split; d.kb_per_split = q.kb_per_split;
     d.first_unit = static_cast<int>(units);
     units += 1ll * d.tiles_m * d.tiles_n * d.split_k;
     if (units > 0x3fffffffll) return -1;
     d.a_mn = q.a_mn ? 1 : 0; d.b_mn = q.b_mn ? 1 : 0;
-    const bool atom32 = l.in.kind == kKindTf32;
+    const MapSwizzle mn_swz = l.in.kind == kKindTf32 ? kSwz128Atom32 : kSwz128;
     for (int j = 0; j < 2; ++j) {
       if (q.a[j].rows > 0)
         ok = ok && encode_narrow(&d.a[j], l.in, q.a[j].p, q.a[j].cols, q.a[j].rows, 1, q.a[j].ld * l.in.bytes,
-                                 q.a[j].ld * l.in.bytes * q.a[j].rows, kblock, q.a_mn ? kblock : 128, q.a_mn && atom32);
+                                 q.a[j].ld * l.in.bytes * q.a[j].rows, kblock, q.a_mn ? kblock : 128,
+                                 q.a_mn ? mn_swz : kSwz128);
       if (q.b[j].rows > 0)
         ok = ok && encode_narrow(&d.b[j], l.in, q.b[j].p, q.b[j].cols, q.b[j].rows, 1, q.b[j].ld * l.in.bytes,
-                                 q.b[j].ld * l.in.bytes * q.b[j].rows, kblock, q.b_mn ? kblock : half_n, q.b_mn && atom32);
+                                 q.b[j].ld * l.in.bytes * q.b[j].rows, kblock, q.b_mn ? kblock : half_n,
+                                 q.b_mn ? mn_swz : kSwz128);
+      if (q.aux[j] != nullptr)
+        ok = ok && encode_narrow(&d.aux[j], out, q.aux[j], q.n, q.m, 1, q.aux_ld * out.bytes,
+                                 q.aux_ld * out.bytes * q.m, 32, 32, out_swz);
     }
     if (q.split > 1) {
       const long long ld = partial_ld(q);
-      d.out_ptr[0] = q.partials;
       d.tma_out[0] = 1;
-      ok = ok && encode_narrow(&d.out[0], f32, q.partials, q.n, q.m, q.split, ld * 4, ld * 4 * q.m, 32, 32, false);
+      ok = ok && encode_narrow(&d.out[0], f32, q.partials, q.n, q.m, q.split, ld * 4, ld * 4 * q.m, 32, 32, kSwz128);
     } else {
       for (int j = 0; j < 3; ++j) {
         if (q.out[j] == nullptr) continue;
@@ -360,30 +396,28 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
         d.tma_out[j] = rows_addressable(q.out[j], q.out_ld[j], out.bytes) ? 1 : 0;
         if (d.tma_out[j])
           ok = ok && encode_narrow(&d.out[j], out, q.out[j], q.n, q.m, 1, q.out_ld[j] * out.bytes,
-                                   q.out_ld[j] * out.bytes * q.m, 128 / out.bytes, 32, false);
+                                   q.out_ld[j] * out.bytes * q.m, 32, 32, out_swz);
       }
     }
-    d.gate = q.gate; d.up = q.up; d.aux_ld = q.aux_ld;
   }
   if (!ok) return -1;
   p.count = count;
   p.total_units = static_cast<int>(units);
-  p.block_n = plan.block_n;
-  const size_t stage = kNarrowABytes + half_n * 128;
-  int stages = static_cast<int>((kMaxDynSmem - narrow_pair_smem_bytes(plan.block_n, 0)) / stage);
+  const size_t stage = kNarrowABytes + static_cast<size_t>(p.groups) * half_n * 128;
+  const size_t fixed = narrow_fixed_bytes(l.epi);
+  const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
   p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;
   p.group_m = 8;
   p.act = l.act;
   p.is_bf16 = l.in.code == FASTNN_B200_BF16 ? 1 : 0;
   p.row_scale = l.row_scale; p.col_scale = l.col_scale; p.col_scale2 = l.col_scale2; p.bias = l.bias;
+  p.vec_scale = aligned16(l.col_scale) && aligned16(l.col_scale2) && aligned16(l.bias) ? 1 : 0;
   p.status = st->status;
   p.spin_budget = st->spin_budget;
   const int clusters = p.total_units < st->max_clusters ? p.total_units : st->max_clusters;
-  NarrowKernel k = pair_kernel(l.in.kind, l.epi, l.out_code);
+  const NarrowKernel<N> k = pair_kernel<N>(l.in.kind, l.epi, l.out_code);
   if (k == nullptr || clusters < 1) return -1;
-  k<<<2 * clusters, kNarrowThreads, narrow_pair_smem_bytes(p.block_n, p.num_stages), stream>>>(p);
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  FNN_CUDA_OK(cudaGetLastError());
+  if (launch_dependent(k, 2 * clusters, kNarrowThreads, fixed + p.num_stages * stage, stream, p) != 0) return -1;
   t_last = LastCall{12, plan.block_n, t[0].split, 2 * clusters};
 
   NarrowReduceParams r;
@@ -404,11 +438,9 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   if (blocks > 0) {
     if (blocks > 0x7fffffffll) return -1;
     const unsigned g = static_cast<unsigned>(blocks);
-    if (l.out_code == FASTNN_B200_F32) narrow_reduce_kernel<float><<<g, 256, 0, stream>>>(r);
-    else if (l.out_code == FASTNN_B200_BF16) narrow_reduce_kernel<__nv_bfloat16><<<g, 256, 0, stream>>>(r);
-    else narrow_reduce_kernel<__half><<<g, 256, 0, stream>>>(r);
-    g_launches.fetch_add(1, std::memory_order_relaxed);
-    FNN_CUDA_OK(cudaGetLastError());
+    auto* k = l.out_code == FASTNN_B200_F32 ? narrow_reduce_kernel<float>
+              : (l.out_code == FASTNN_B200_BF16 ? narrow_reduce_kernel<__nv_bfloat16> : narrow_reduce_kernel<__half>);
+    if (launch_dependent(k, g, 256, 0, stream, r) != 0) return -1;
   }
   return 0;
 }
@@ -442,10 +474,10 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
   const int tiles = ceil_div(t.n, tile_rows);
   p.split = skinny_split(tiles, p.num_kb);
   bool ok = encode_narrow(&p.x, l.in, t.a[0].p, t.a[0].cols, t.a[0].rows, 1, t.a[0].ld * l.in.bytes,
-                          t.a[0].ld * l.in.bytes * t.a[0].rows, kblock, p.n_mma, false);
+                          t.a[0].ld * l.in.bytes * t.a[0].rows, kblock, p.n_mma, kSwz128);
   for (int j = 0; j < (two ? 2 : 1); ++j)
     ok = ok && encode_narrow(&p.w[j], l.in, t.b[j].p, t.b[j].cols, t.b[j].rows, 1, t.b[j].ld * l.in.bytes,
-                             t.b[j].ld * l.in.bytes * t.b[j].rows, kblock, tile_rows, false);
+                             t.b[j].ld * l.in.bytes * t.b[j].rows, kblock, tile_rows, kSwz128);
   if (!ok) return -1;
   DType out;
   if (!dtype_of(l.out_code, &out)) return -1;
@@ -550,15 +582,15 @@ int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cu
     return launch_skinny(st, l, t2, true, s);
   }
   const int cl = clusters_of(st);
-  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, true, false);
-  const NarrowPlan p2 = plan_narrow(&t2, 1, kblock, cl, false, true);
+  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGated, false);
+  const NarrowPlan p2 = plan_narrow(&t2, 1, kblock, cl, fnn::kEpiStore, true);
   reserve_partials(ws, &t2, 1);
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
-  if (launch_pair(st, l, &t1, 1, p1, s) != 0) return -1;
+  if (launch_pair<1>(st, l, &t1, 1, p1, s) != 0) return -1;
   l.epi = fnn::kEpiStore;
-  return launch_pair(st, l, &t2, 1, p2, s);
+  return launch_pair<1>(st, l, &t2, 1, p2, s);
 }
 
 int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cudaStream_t s) {
@@ -589,7 +621,7 @@ int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, c
   t1.m = a.rows; t1.n = a.f; t1.k = a.d;
   t1.out[0] = dg; t1.out[1] = du; t1.out[2] = h;
   for (long long& ld : t1.out_ld) ld = h_ld;
-  t1.gate = gate.p; t1.up = up.p; t1.aux_ld = gate.ld;
+  t1.aux[0] = gate.p; t1.aux[1] = up.p; t1.aux_ld = gate.ld;
 
   NarrowTask g[4];
   g[0].a[0] = mdg; g[0].a[1] = mdu; g[0].b[0] = wg; g[0].b[1] = wu;       // dx
@@ -607,16 +639,16 @@ int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, c
   g[3].m = a.d; g[3].n = a.f; g[3].k = a.rows;
   g[3].out[0] = a.dwd; g[3].out_ld[0] = a.f;
   const int cl = clusters_of(st);
-  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, false, false);
-  const NarrowPlan p2 = plan_narrow(g, 4, kblock, cl, false, true);
+  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGatedGrad, false);
+  const NarrowPlan p2 = plan_narrow(g, 4, kblock, cl, fnn::kEpiStore, true);
   reserve_partials(ws, g, 4);
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
   NarrowLaunch l{a.t, a.t.code, fnn::kEpiGatedGrad, a.act};
-  if (launch_pair(st, l, &t1, 1, p1, s) != 0) return -1;
+  if (launch_pair<1>(st, l, &t1, 1, p1, s) != 0) return -1;
   l.epi = fnn::kEpiStore;
-  return launch_pair(st, l, g, 4, p2, s);
+  return launch_pair<fnn::kNarrowMaxProblems>(st, l, g, 4, p2, s);
 }
 
 bool ffn_sizes_ok(int rows, int d, int f) { return rows >= 0 && d >= 1 && f >= 1; }
@@ -657,8 +689,8 @@ int int8_product(DeviceState* st, const Int8Args& a, Carver& ws, bool pack_all, 
   NarrowLaunch l{kInt8, a.out_code, a.gated ? fnn::kEpiScaledGated : fnn::kEpiScaled, a.act};
   l.row_scale = a.xs; l.col_scale = a.ws; l.col_scale2 = a.ws2; l.bias = a.bias;
   if (use_skinny(a.rows)) return launch_skinny(st, l, t, false, s);
-  const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), a.gated, false);
-  return launch_pair(st, l, &t, 1, p, s);
+  const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), l.epi, false);
+  return launch_pair<1>(st, l, &t, 1, p, s);
 }
 
 // INT32 accumulators hold sums of k products of magnitude at most 128 * 128.
@@ -674,13 +706,9 @@ int quantize_launch(const void* x, long long ld, int8_t* q, float* scale, int ro
   const bool warp = cols <= 32 * kQuantHeld * v;
   const int per = kQuantThreads / 32;
   const int grid = warp ? (rows + per - 1) / per : rows;
-  if (warp && vec) quantize_rows_kernel<T, 32, true><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
-  else if (warp) quantize_rows_kernel<T, 32, false><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
-  else if (vec) quantize_rows_kernel<T, kQuantThreads, true><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
-  else quantize_rows_kernel<T, kQuantThreads, false><<<grid, kQuantThreads, 0, s>>>(src, ld, q, scale, rows, cols);
-  g_launches.fetch_add(1, std::memory_order_relaxed);
-  FNN_CUDA_OK(cudaGetLastError());
-  return 0;
+  auto* k = warp ? (vec ? quantize_rows_kernel<T, 32, true> : quantize_rows_kernel<T, 32, false>)
+                 : (vec ? quantize_rows_kernel<T, kQuantThreads, true> : quantize_rows_kernel<T, kQuantThreads, false>);
+  return launch_dependent(k, static_cast<unsigned>(grid), kQuantThreads, 0, s, src, ld, q, scale, rows, cols);
 }
 
 }  // namespace

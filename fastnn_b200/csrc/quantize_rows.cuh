@@ -45,6 +45,8 @@ template <typename T, int kPerRow, bool kVec>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* __restrict__ x, long long ld,
                                                                       int8_t* __restrict__ q,
                                                                       float* __restrict__ scale, int rows, int cols) {
+  ptx::grid_dep_wait();
+  ptx::grid_dep_launch_dependents();
   constexpr int kV = kVec ? 16 / static_cast<int>(sizeof(T)) : 1;
   const int part = threadIdx.x % kPerRow;
   const long long row = static_cast<long long>(blockIdx.x) * (kQuantThreads / kPerRow) + threadIdx.x / kPerRow;
