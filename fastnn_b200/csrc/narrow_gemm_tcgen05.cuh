@@ -37,22 +37,43 @@ enum : int {
 // Activations of this file's epilogues (the public codes, kActSilu beyond the GEMM epilogue's own).
 constexpr int kActSilu = 5;
 
-constexpr int kNarrowEpiWarps = 8;
-constexpr int kNarrowMmaWarpB = 2 + kNarrowEpiWarps; // second MMA-issuing warp (wide tiles)
-constexpr int kNarrowThreads = 32 * (kNarrowMmaWarpB + 1);
+// Epilogue warps, four for each TMEM lane quadrant: what an epilogue waits for (tensor memory, staging
+// tiles, fixed latencies) is covered by other warps, and with two for each quadrant a tile's drain took
+// 1.5 to 2 times as long (7.2 against 4 k clocks for 256 columns of 8-bit products).  The gradient
+// epilogue is bound by its memory traffic and has two with two sets of tiles each.
+template <int kEpi>
+constexpr int kEpiWarps = kEpi == kEpiGatedGrad ? 8 : 16;
+template <int kEpi>
+constexpr int kNarrowThreads = 32 * (kEpiWarps<kEpi> + 3);    // + producer and two MMA issuers
 constexpr int kNarrowMaxProblems = 4;
 constexpr int kNarrowMaxStages = 8;
 constexpr int kNarrowABytes = 128 * 128;             // 128 rows x 128 bytes of K
 constexpr int kNarrowBarBytes = 512;
-// Staging tiles: 32 rows x 32 columns of the output type, rows of 64 (16-bit) or 128 bytes in the
-// swizzle of that span.
+constexpr int kNarrowGroupM = 8;                     // tile rows of a rasterisation group: 2048 rows
+// A staging tile is 32 rows of 64 bytes (in the 64-byte swizzle): 32 columns of 16 bits, 16 of 32.  An
+// epilogue warp owns one; a gradient epilogue's owns two sets of (gate, up, h).
+constexpr int kTile = 32 * 64;
 template <typename T>
-constexpr int kTileBytes = 32 * 32 * static_cast<int>(sizeof(T));
-// Staging bytes of one epilogue warp.  Two tiles in turn, of which one is being stored while the next is
-// filled; a gradient epilogue holds sets of (gate, up, h) tiles instead, two of 16 bits or one of 32.
-// The FP32 partial sums of a K split need 4 KiB of either.
-template <int kEpi, typename T>
-constexpr int kStagingWarp = kEpi == kEpiGatedGrad ? 12288 : 4096;
+constexpr int kTileCols = 64 / static_cast<int>(sizeof(T));
+template <int kEpi>
+constexpr int kStagingWarp = kEpi == kEpiGatedGrad ? 6 * kTile : kTile;
+
+// n / d for 0 <= n < 2^31 without a division (Granlund and Montgomery): every epilogue warp decodes every
+// tile, and four integer divisions were a third of a short-K tile's instructions.
+struct FastDiv {
+  uint32_t mul, shift, d;
+};
+inline FastDiv fast_div(int d) {
+  FastDiv f;
+  f.d = static_cast<uint32_t>(d);
+  f.shift = 0;
+  while ((1ull << f.shift) < f.d) ++f.shift;
+  f.mul = static_cast<uint32_t>(((1ull << 32) * ((1ull << f.shift) - f.d)) / f.d + 1);
+  return f;
+}
+__device__ __forceinline__ int div_by(int n, const FastDiv& f) {
+  return static_cast<int>((__umulhi(static_cast<uint32_t>(n), f.mul) + static_cast<uint32_t>(n)) >> f.shift);
+}
 
 struct NarrowProblem {
   CUtensorMap a[2], b[2];      // [1]: second K range (C = A0.B0 + A1.B1), or the up weight of a gated product
@@ -66,6 +87,8 @@ struct NarrowProblem {
   int num_kb, num_kb1;         // 128-byte k-blocks in all, and those of the first operand pair
   int split_k, kb_per_split;   // split_k > 1: partial sums, FP32, one [m, n] block per slice in out[0]
   int first_unit;
+  int full_groups;             // rasterisation groups of group_m tile rows
+  FastDiv by_split, by_group, by_rows, by_last;   // K slices; tiles of a full group; tile rows of a group, of the last
   int a_mn, b_mn;              // operand stored with M (N) contiguous
 };
 
@@ -137,15 +160,36 @@ __device__ __forceinline__ uint64_t narrow_desc(uint32_t addr, int mn_major) {
 }
 
 // ------------------------------------------------------------------ activations ---
-// x / (1 + e^-x) on the special-function unit: __expf and __fdividef are good to a few units in
-// the last place of FP32 where the result is a normal number.
-__device__ __forceinline__ float silu(float x) { return __fdividef(x, 1.0f + __expf(-x)); }
+// These run over every output of a tile while the next tile's main loop wants to start, so they are
+// written for few instructions: the special-function unit's 2^x and 1/x (a unit or two in the last
+// place of FP32) and no range handling beyond what the formulas need.
+constexpr float kLog2e = 1.4426950408889634f;
+
+// 1 / (1 + e^-x).  e^-x overflows to infinity below x = -88, where 1 / inf = 0 stands for e^x < 1e-38.
+__device__ __forceinline__ float sigmoid_fast(float x) {
+  return ptx::rcp_approx(1.0f + ptx::ex2_approx(x * -kLog2e));
+}
+
+// The normal distribution's Phi(x) = 0.5 erfc(-x / sqrt 2), and e^(-x^2 / 2) beside it.  erfc by
+// Abramowitz & Stegun 7.1.26, erfc(z) = (a1 t + ... + a5 t^5) e^(-z^2) with t = 1 / (1 + 0.3275911 z),
+// z >= 0: off by at most 1.5e-7.  The tail is computed as itself, not as 1 - erf, so Phi keeps that
+// accuracy's size for negative x.  About half the instructions of erff.
+__device__ __forceinline__ float normal_cdf(float x, float& gauss) {
+  const float t = ptx::rcp_approx(fmaf(fabsf(x), 0.3275911f * 0.7071067811865475f, 1.0f));
+  gauss = ptx::ex2_approx(x * x * (-0.5f * kLog2e));
+  float q = fmaf(t, 0.5f * 1.061405429f, 0.5f * -1.453152027f);
+  q = fmaf(t, q, 0.5f * 1.421413741f);
+  q = fmaf(t, q, 0.5f * -0.284496736f);
+  q = fmaf(t, q, 0.5f * 0.254829592f);
+  q *= t * gauss;
+  return x >= 0.0f ? 1.0f - q : q;
+}
 
 template <int kAct>
 __device__ __forceinline__ float gate_act(float x) {
   if constexpr (kAct == kActRelu) return x < 0.0f ? 0.0f : x;        // NaN stays NaN
-  else if constexpr (kAct == kActGelu) return gelu_erf(x);
-  else if constexpr (kAct == kActSilu) return silu(x);
+  else if constexpr (kAct == kActGelu) { float e; return x * normal_cdf(x, e); }
+  else if constexpr (kAct == kActSilu) return x * sigmoid_fast(x);
   else return x;
 }
 // act(x) and its derivative together
@@ -155,11 +199,12 @@ __device__ __forceinline__ void gate_act_grad(float x, float& a, float& da) {
     a = x < 0.0f ? 0.0f : x;
     da = x > 0.0f ? 1.0f : 0.0f;
   } else if constexpr (kAct == kActGelu) {
-    const float cdf = 0.5f * (1.0f + erff(x * 0.7071067811865475f));
+    float e;
+    const float cdf = normal_cdf(x, e);
     a = x * cdf;
-    da = fmaf(x, __expf(-0.5f * x * x) * 0.3989422804014327f, cdf);
+    da = fmaf(x * 0.3989422804014327f, e, cdf);
   } else if constexpr (kAct == kActSilu) {
-    const float s = __fdividef(1.0f, 1.0f + __expf(-x));
+    const float s = sigmoid_fast(x);
     a = x * s;
     da = s * fmaf(x, 1.0f - s, 1.0f);
   } else {
@@ -192,41 +237,22 @@ __device__ __forceinline__ float2 unpack2<__half>(uint32_t v) {
   return __half22float2(*reinterpret_cast<const __half2*>(&v));
 }
 
-// Byte offset of 16-byte unit j of row r in a staging tile: rows of 64 bytes in the 64-byte swizzle
-// (unit j at j ^ ((r >> 1) & 3)), rows of 128 in the 128-byte one (j ^ (r & 7)).
-template <typename T>
+// Byte offset of 16-byte unit j of row r in a staging tile: unit j at j ^ ((r >> 1) & 3).
 __device__ __forceinline__ uint32_t tile_unit(int r, int j) {
-  if constexpr (sizeof(T) == 4) return static_cast<uint32_t>(r * 128 + ((j ^ (r & 7)) << 4));
-  else return static_cast<uint32_t>(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
+  return static_cast<uint32_t>(r * 64 + ((j ^ ((r >> 1) & 3)) << 4));
 }
 
-// This lane's row, 32 columns, to and from a staging tile.
-template <typename T>
-__device__ __forceinline__ void tile_put(uint8_t* tile, int lane, const float (&v)[32]) {
-  if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      *reinterpret_cast<float4*>(tile + tile_unit<T>(lane, j)) =
-          make_float4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      *reinterpret_cast<uint4*>(tile + tile_unit<T>(lane, j)) =
-          make_uint4(pack2<T>(v[8 * j], v[8 * j + 1]), pack2<T>(v[8 * j + 2], v[8 * j + 3]),
-                     pack2<T>(v[8 * j + 4], v[8 * j + 5]), pack2<T>(v[8 * j + 6], v[8 * j + 7]));
-  }
-}
-// 8 columns of it: the j-th eighth (32-bit types: two units) or unit j
+// 8 columns of this lane's row to and from a staging tile: the j-th eight (a unit of 16 bits, two of 32).
 template <typename T>
 __device__ __forceinline__ void tile_get8(const uint8_t* tile, int lane, int j, float (&v)[8]) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float4 f = *reinterpret_cast<const float4*>(tile + tile_unit<T>(lane, 2 * j + i));
+      const float4 f = *reinterpret_cast<const float4*>(tile + tile_unit(lane, 2 * j + i));
       v[4 * i] = f.x; v[4 * i + 1] = f.y; v[4 * i + 2] = f.z; v[4 * i + 3] = f.w;
     }
   } else {
-    const uint4 w = *reinterpret_cast<const uint4*>(tile + tile_unit<T>(lane, j));
+    const uint4 w = *reinterpret_cast<const uint4*>(tile + tile_unit(lane, j));
     const uint32_t q[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -236,38 +262,47 @@ __device__ __forceinline__ void tile_get8(const uint8_t* tile, int lane, int j, 
   }
 }
 template <typename T>
-__device__ __forceinline__ void tile_put8(uint8_t* tile, int lane, int j, const float (&v)[8]) {
+__device__ __forceinline__ void tile_put8(uint8_t* tile, int lane, int j, const float* v) {
   if constexpr (sizeof(T) == 4) {
 #pragma unroll
     for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<float4*>(tile + tile_unit<T>(lane, 2 * j + i)) =
+      *reinterpret_cast<float4*>(tile + tile_unit(lane, 2 * j + i)) =
           make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
   } else {
-    *reinterpret_cast<uint4*>(tile + tile_unit<T>(lane, j)) =
+    *reinterpret_cast<uint4*>(tile + tile_unit(lane, j)) =
         make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
   }
+}
+// 16 columns, the h-th sixteen
+template <typename T>
+__device__ __forceinline__ void tile_put16(uint8_t* tile, int lane, int h, const float (&v)[16]) {
+  tile_put8<T>(tile, lane, 2 * h, v);
+  tile_put8<T>(tile, lane, 2 * h + 1, v + 8);
 }
 
 // A staging tile to output rows [m0, m0 + 32), columns from col0: one TMA store, which clips at the
 // matrix's edges, or row by row (row strides that are no multiple of 16 bytes, unaligned bases).
 template <typename T>
 __device__ __forceinline__ void tile_flush(const CUtensorMap* map, void* out, long long ld, int tma, uint8_t* tile,
-                                           uint32_t tile_addr, int m0, int col0, int z, int m, int n, int lane) {
+                                           uint32_t tile_addr, int m0, int col0, int m, int n, int lane) {
   if (tma) {
     ptx::fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      ptx::tma_store_3d(map, tile_addr, col0, m0, z);
+      ptx::tma_store_3d(map, tile_addr, col0, m0, 0);
       ptx::tma_store_commit();
     }
   } else {
     __syncwarp();
     const int rows = min(32, m - m0);
-    T* dst = static_cast<T*>(out) + static_cast<long long>(m0) * ld + col0 + lane;
     constexpr int kPer = 16 / static_cast<int>(sizeof(T));
-    if (col0 + lane < n)
-      for (int r = 0; r < rows; ++r)
-        dst[r * ld] = *reinterpret_cast<const T*>(tile + tile_unit<T>(r, lane / kPer) + (lane % kPer) * sizeof(T));
+    // lanes over the columns of as many rows at once as fit the warp
+    constexpr int kRowsAtOnce = 32 / kTileCols<T>;
+    const int cl = lane % kTileCols<T>;
+    T* dst = static_cast<T*>(out) + static_cast<long long>(m0) * ld + col0 + cl;
+    if (col0 + cl < n)
+      for (int r = lane / kTileCols<T>; r < rows; r += kRowsAtOnce)
+        dst[r * ld] = *reinterpret_cast<const T*>(tile + tile_unit(r, cl / kPer) + (cl % kPer) * sizeof(T));
     __syncwarp();
   }
 }
@@ -313,22 +348,20 @@ __device__ __forceinline__ NarrowUnit narrow_unit(const NarrowParams<kProblems>&
   const NarrowProblem& q = p.pr[i];
   int t = u - q.first_unit;
   w.pr = i;
-  w.s = t % q.split_k;
-  t /= q.split_k;
-  const int group_sz = p.group_m * q.tiles_n;
-  const int g = t / group_sz;
-  const int first_m = g * p.group_m;
-  const int gm = min(q.tiles_m - first_m, p.group_m);
-  const int r = t - g * group_sz;
-  w.mt = first_m + r % gm;
-  w.nt = r / gm;
+  const int tile = div_by(t, q.by_split);
+  w.s = t - tile * q.split_k;
+  const int g = div_by(tile, q.by_group);
+  const int r = tile - g * static_cast<int>(q.by_group.d);
+  const FastDiv& rows = g < q.full_groups ? q.by_rows : q.by_last;
+  w.nt = div_by(r, rows);
+  w.mt = g * p.group_m + r - w.nt * static_cast<int>(rows.d);
   w.kb0 = w.s * q.kb_per_split;
   w.kb1 = min(q.num_kb, w.kb0 + q.kb_per_split);
   return w;
 }
 
 template <int kKind, int kEpi, typename OutT, int kProblems>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNarrowThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNarrowThreads<kEpi>, 1)
 narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   using K = NarrowKind<kKind>;
   constexpr bool kTwoB = kEpi == kEpiGated || kEpi == kEpiScaledGated;
@@ -348,7 +381,9 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   const uint32_t half_bytes = static_cast<uint32_t>(half_n) * 128u;
   const uint32_t stage_bytes = kNarrowABytes + static_cast<uint32_t>(groups) * half_bytes;
   const uint32_t staging_base = smem_base + p.num_stages * stage_bytes;
-  const uint32_t bar_base = staging_base + kNarrowEpiWarps * kStagingWarp<kEpi, OutT>;
+  constexpr int kWarps = kEpiWarps<kEpi>;
+  constexpr int kMmaWarpB = 2 + kWarps;                  // second MMA-issuing warp (wide tiles)
+  const uint32_t bar_base = staging_base + kWarps * kStagingWarp<kEpi>;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 64u + 8u * s; };
   auto tfull_bar = [&](int a) { return bar_base + 128u + 8u * a; };
@@ -366,10 +401,10 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
     }
     for (int a = 0; a < 2; ++a) {
       ptx::mbar_init(tfull_bar(a), 1);
-      ptx::mbar_init(tempty_bar(a), 2 * kNarrowEpiWarps);
+      ptx::mbar_init(tempty_bar(a), 2 * kWarps);
     }
     if constexpr (kGrad)
-      for (int i = 0; i < 2 * kNarrowEpiWarps; ++i) ptx::mbar_init(bar_base + 256u + 8u * i, 1);
+      for (int i = 0; i < 2 * kWarps; ++i) ptx::mbar_init(bar_base + 256u + 8u * i, 1);
     *abort_flag = 0;
     ptx::fence_mbar_init();
     ptx::fence_proxy_async_smem();
@@ -443,7 +478,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
         if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
       }
     }
-  } else if (warp == 1 || warp == kNarrowMmaWarpB) {
+  } else if (warp == 1 || warp == kMmaWarpB) {
     // ----------------------------------------------- MMA issuers (leader only) ---
     // One thread per MMA group.  The two accumulator slots of 256 columns hold alternate tiles of a
     // one-group launch, or the two groups of a wide tile; either way a slot is filled again as soon as
@@ -494,21 +529,19 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
     }
   } else {
     // -------------------------------------------------------------- epilogue ---
-    // Two warps per TMEM lane quadrant take alternate 32-column chunks of a slot.
+    // The warps of a TMEM lane quadrant take the column chunks of a slot in turn; a chunk fills a tile.
     const int ew = warp - 2;
     const int q4 = warp & 3;
     const int group = ew >> 2;
-    const uint32_t my_addr = staging_base + ew * kStagingWarp<kEpi, OutT>;
+    constexpr int kStep = kWarps / 4;
+    constexpr int kCols = kTileCols<OutT>;
+    const uint32_t my_addr = staging_base + ew * kStagingWarp<kEpi>;
     uint8_t* my_gen = smem_gen + (my_addr - smem_base);
-    constexpr int kTile = kTileBytes<OutT>;
-    constexpr int kBufs = kStagingWarp<kEpi, OutT> / kTile < 2 ? 1 : 2;
-    int buf = 0;
     int slot = 0;
     uint32_t slot_phase = 0;
     bool ok = true;
 
     // kGrad: the (gate, up) tiles of the next chunk are fetched while this one is computed
-    constexpr int kSets = kGrad ? kStagingWarp<kEpi, OutT> / (3 * kTile) : 1;
     int set = 0;
     uint32_t set_phase = 0;                                  // a bit for each set
     bool fetched = false;                                    // the current set's tiles are on their way
@@ -517,7 +550,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
       if constexpr (kGrad) {
         const NarrowProblem& q = p.pr[w.pr];
         const int m0 = w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32;
-        const int col0 = w.nt * block_n + c * 32;
+        const int col0 = w.nt * block_n + c * kCols;
         const uint32_t bar = aux_bar(ew, s);
         ptx::mbar_expect_tx(bar, 2 * kTile);
         ptx::tma_load_3d(set_addr(s), &q.aux[0], bar, col0, m0, 0);
@@ -527,7 +560,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
     // whether chunk c of unit u exists for this warp (its rows and columns reach into the matrix)
     auto live = [&](const NarrowUnit& w, int c) {
       const NarrowProblem& q = p.pr[w.pr];
-      return w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32 < q.m && w.nt * block_n + c * 32 < q.n;
+      return w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32 < q.m && w.nt * block_n + c * kCols < q.n;
     };
     if constexpr (kGrad) {
       const NarrowUnit w = narrow_unit(p, cluster_id);       // the grid has no more pairs than units
@@ -549,105 +582,120 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
         ptx::tc_fence_after_sync();
         const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q4 * 32) << 16) +
                                static_cast<uint32_t>(slot * kMaxBlockN);
-        auto load32 = [&](int col, uint32_t (&r)[32]) { ptx::tmem_ld_32x32(taddr + col, r); };
+        auto load16 = [&](int col, uint32_t (&r)[16]) { ptx::tmem_ld_32x16(taddr + col, r); };
         auto value = [&](uint32_t r) {
           return kKind == kKindI8 ? static_cast<float>(static_cast<int>(r)) : __uint_as_float(r);
         };
-        auto next_tile = [&]() {                             // a staging tile that may be overwritten
-          if constexpr (kBufs == 2) buf ^= 1;
-          if (lane == 0) ptx::tma_store_wait_read<kBufs - 1>();
+        auto tile_free = [&]() {                             // the staging tile may be overwritten
+          if (lane == 0) ptx::tma_store_wait_read<0>();
           __syncwarp();
+        };
+        auto flush = [&](int i, int col0) {
+          tile_flush<OutT>(&q.out[i], q.out_ptr[i], q.out_ld[i], q.tma_out[i], my_gen, my_addr, m0, col0, q.m, q.n, lane);
         };
         if (rows_live) {
           if constexpr (kEpi == kEpiStore) {
             const int n0 = w.nt * block_n + g * p.mma_n;
             if (raw) {                                       // FP32 partial sums of one K slice
-              for (int c = group; c < p.mma_n / 32; c += 2) {
-                const int col0 = n0 + c * 32;
+              for (int c = group; c < p.mma_n / 16; c += kStep) {
+                const int col0 = n0 + c * 16;
                 if (col0 >= q.n) break;
-                uint32_t r[32];
-                load32(c * 32, r);
-                if (lane == 0) ptx::tma_store_wait_read<0>();
-                __syncwarp();
+                uint32_t r[16];
+                load16(c * 16, r);
+                tile_free();
                 ptx::tmem_ld_wait();
-                float v[32];
+                float v[16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-                tile_put<float>(my_gen, lane, v);
-                tile_flush<float>(&q.out[0], nullptr, 0, 1, my_gen, my_addr, m0, col0, w.s, q.m, q.n, lane);
+                for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                tile_put16<float>(my_gen, lane, 0, v);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  ptx::tma_store_3d(&q.out[0], my_addr, col0, m0, w.s);
+                  ptx::tma_store_commit();
+                }
               }
             } else {
-              for (int c = group; c < p.mma_n / 32; c += 2) {
-                const int col0 = n0 + c * 32;
+              for (int c = group; c < p.mma_n / kCols; c += kStep) {
+                const int col0 = n0 + c * kCols;
                 if (col0 >= q.n) break;
-                uint32_t r[32];
-                load32(c * 32, r);
-                next_tile();
-                ptx::tmem_ld_wait();
-                float v[32];
+                uint32_t r[kCols / 16][16];
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
-                tile_put<OutT>(my_gen + buf * kTile, lane, v);
-                tile_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], my_gen + buf * kTile,
-                                 my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+                for (int h = 0; h < kCols / 16; ++h) load16(c * kCols + h * 16, r[h]);
+                tile_free();
+                ptx::tmem_ld_wait();
+#pragma unroll
+                for (int h = 0; h < kCols / 16; ++h) {
+                  float v[16];
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[h][j]);
+                  tile_put16<OutT>(my_gen, lane, h, v);
+                }
+                flush(0, col0);
               }
             }
           } else if constexpr (kEpi == kEpiGated) {
             const int n0 = w.nt * (block_n >> 1) + g * half_n;
-            const bool save = q.out_ptr[1] != nullptr;
-            for (int c = group; c < half_n / 32; c += 2) {
-              const int col0 = n0 + c * 32;
+            for (int c = group; c < half_n / kCols; c += kStep) {
+              const int col0 = n0 + c * kCols;
               if (col0 >= q.n) break;
-              uint32_t rg[32], ru[32];
-              load32(c * 32, rg);
-              load32(half_n + c * 32, ru);
-              next_tile();
-              ptx::tmem_ld_wait();
-              float gv[32], v[32];
+              if (q.out_ptr[1] != nullptr) {                 // the projections themselves, for the backward pass
+                for (int i = 0; i < 2; ++i) {
+                  tile_free();
 #pragma unroll
-              for (int j = 0; j < 32; ++j) { gv[j] = __uint_as_float(rg[j]); v[j] = __uint_as_float(ru[j]); }
-              if (save) {                                    // the projections themselves, for the backward pass
-                tile_put<OutT>(my_gen + buf * kTile, lane, gv);
-                tile_flush<OutT>(&q.out[1], q.out_ptr[1], q.out_ld[1], q.tma_out[1], my_gen + buf * kTile,
-                                 my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
-                next_tile();
-                tile_put<OutT>(my_gen + buf * kTile, lane, v);
-                tile_flush<OutT>(&q.out[2], q.out_ptr[2], q.out_ld[2], q.tma_out[2], my_gen + buf * kTile,
-                                 my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
-                next_tile();
+                  for (int h = 0; h < kCols / 16; ++h) {
+                    uint32_t r[16];
+                    load16(i * half_n + c * kCols + h * 16, r);
+                    ptx::tmem_ld_wait();
+                    float v[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+                    tile_put16<OutT>(my_gen, lane, h, v);
+                  }
+                  flush(1 + i, col0);
+                }
               }
-              for_act(p.act, [&](auto tag) {
-                constexpr int kAct = decltype(tag)::value;
+              tile_free();
 #pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] *= gate_act<kAct>(gv[j]);
-              });
-              tile_put<OutT>(my_gen + buf * kTile, lane, v);
-              tile_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], my_gen + buf * kTile,
-                               my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+              for (int h = 0; h < kCols / 16; ++h) {
+                uint32_t rg[16], ru[16];
+                load16(c * kCols + h * 16, rg);
+                load16(half_n + c * kCols + h * 16, ru);
+                ptx::tmem_ld_wait();
+                float v[16];
+                for_act(p.act, [&](auto tag) {
+                  constexpr int kAct = decltype(tag)::value;
+#pragma unroll
+                  for (int j = 0; j < 16; ++j)
+                    v[j] = gate_act<kAct>(__uint_as_float(rg[j])) * __uint_as_float(ru[j]);
+                });
+                tile_put16<OutT>(my_gen, lane, h, v);
+              }
+              flush(0, col0);
             }
           } else if constexpr (kGrad) {
             // dgate and dup take the places of gate and up in the set's tiles (a lane reads and writes
             // its own row), h a third tile; all three rows are addressable by construction
             const int n0 = w.nt * block_n;
-            for (int c = group; c < block_n / 32; c += 2) {
-              const int col0 = n0 + c * 32;
+            for (int c = group; c < block_n / kCols; c += kStep) {
+              const int col0 = n0 + c * kCols;
               if (col0 >= q.n) break;
-              uint32_t r[32];
-              load32(c * 32, r);
+              uint32_t r[kCols / 16][16];
+#pragma unroll
+              for (int h = 0; h < kCols / 16; ++h) load16(c * kCols + h * 16, r[h]);
               uint8_t* tiles = my_gen + set * 3 * kTile;
               NarrowUnit wn = w;                             // the chunk this warp comes to next
-              int cn = c + 2;
-              bool more = cn * 32 < block_n && live(wn, cn);
+              int cn = c + kStep;
+              bool more = cn * kCols < block_n && live(wn, cn);
               if (!more && u + num_clusters < p.total_units) {
                 wn = narrow_unit(p, u + num_clusters);
                 cn = group;
                 more = live(wn, cn);
               }
               if (lane == 0) {
-                // every store so far has read its tiles: these may be filled again
-                if (!fetched || kSets == 2) ptx::tma_store_wait_read<0>();
+                ptx::tma_store_wait_read<0>();               // every store so far has read its tiles
                 if (!fetched) fetch_aux(w, c, set);
-                if (kSets == 2 && more) fetch_aux(wn, cn, set ^ 1);
+                if (more) fetch_aux(wn, cn, set ^ 1);
               }
               __syncwarp();
               ok = narrow_wait(aux_bar(ew, set), (set_phase >> set) & 1u, abort_flag, p, kStatusEpilogueTimeout);
@@ -658,7 +706,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
               for_act(p.act, [&](auto tag) {
                 constexpr int kAct = decltype(tag)::value;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < kCols / 8; ++j) {
                   float gv[8], uv[8], hv[8];
                   tile_get8<OutT>(tiles, lane, j, gv);
                   tile_get8<OutT>(tiles + kTile, lane, j, uv);
@@ -666,7 +714,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
                   for (int i = 0; i < 8; ++i) {
                     float a, da;
                     gate_act_grad<kAct>(gv[i], a, da);
-                    const float dh = __uint_as_float(r[8 * j + i]);
+                    const float dh = __uint_as_float(r[j >> 1][(j & 1) * 8 + i]);
                     hv[i] = a * uv[i];
                     gv[i] = dh * uv[i] * da;
                     uv[i] = dh * a;
@@ -684,65 +732,56 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
                 ptx::tma_store_3d(&q.out[1], ta + kTile, col0, m0, 0);
                 ptx::tma_store_3d(&q.out[2], ta + 2 * kTile, col0, m0, 0);
                 ptx::tma_store_commit();
-                if (kSets == 1 && more) {
-                  ptx::tma_store_wait_read<0>();
-                  fetch_aux(wn, cn, 0);
-                }
               }
               fetched = more;
-              if constexpr (kSets == 2) set ^= 1;
+              set ^= 1;
             }
           } else {
-            // 8-bit products: the scale of this lane's row, and the scales (and bias) of the 32 columns,
+            // 8-bit products: the scale of this lane's row, and the scales (and bias) of the columns,
             // which all lanes read from the same addresses
             constexpr bool kGated = kEpi == kEpiScaledGated;
             const float rs = row < q.m ? __ldg(p.row_scale + row) : 0.0f;
             const int width = kGated ? half_n : p.mma_n;
-            const int n0 = w.nt * (kGated ? block_n >> 1 : block_n) + g * width;
-            for (int c = group; c < width / 32; c += 2) {
-              const int col0 = n0 + c * 32;
-              if (col0 >= q.n) break;
-              uint32_t r[32], ru[32];
-              load32(c * 32, r);
-              if constexpr (kGated) load32(half_n + c * 32, ru);
-              next_tile();
-              ptx::tmem_ld_wait();
-              float v[32];
-              const bool whole = p.vec_scale && col0 + 32 <= q.n;
-              auto column4 = [&](const float* src, int j) {
-                if (whole) return __ldg(reinterpret_cast<const float4*>(src + col0) + j);
-                const int k = col0 + 4 * j;
-                return make_float4(k < q.n ? __ldg(src + k) : 0.0f, k + 1 < q.n ? __ldg(src + k + 1) : 0.0f,
-                                   k + 2 < q.n ? __ldg(src + k + 2) : 0.0f, k + 3 < q.n ? __ldg(src + k + 3) : 0.0f);
-              };
+            auto columns16 = [&](const float* src, int col0, float (&to)[16]) {
+              if (src != nullptr && p.vec_scale && col0 + 16 <= q.n) {
 #pragma unroll
-              for (int j = 0; j < 8; ++j) {
-                const float4 cs = column4(p.col_scale, j);
-                if constexpr (kGated) {
-                  const float4 c2 = column4(p.col_scale2, j);
-                  const float x[4] = {c2.x, c2.y, c2.z, c2.w};
-#pragma unroll
-                  for (int i = 0; i < 4; ++i)
-                    ru[4 * j + i] = __float_as_uint(value(ru[4 * j + i]) * (rs * x[i]));
-                  v[4 * j] = value(r[4 * j]) * (rs * cs.x); v[4 * j + 1] = value(r[4 * j + 1]) * (rs * cs.y);
-                  v[4 * j + 2] = value(r[4 * j + 2]) * (rs * cs.z); v[4 * j + 3] = value(r[4 * j + 3]) * (rs * cs.w);
-                } else {
-                  const float4 b = p.bias != nullptr ? column4(p.bias, j) : make_float4(0.f, 0.f, 0.f, 0.f);
-                  v[4 * j] = fmaf(value(r[4 * j]), rs * cs.x, b.x);
-                  v[4 * j + 1] = fmaf(value(r[4 * j + 1]), rs * cs.y, b.y);
-                  v[4 * j + 2] = fmaf(value(r[4 * j + 2]), rs * cs.z, b.z);
-                  v[4 * j + 3] = fmaf(value(r[4 * j + 3]), rs * cs.w, b.w);
+                for (int j = 0; j < 4; ++j) {
+                  const float4 f = __ldg(reinterpret_cast<const float4*>(src + col0) + j);
+                  to[4 * j] = f.x; to[4 * j + 1] = f.y; to[4 * j + 2] = f.z; to[4 * j + 3] = f.w;
                 }
-              }
-              for_act(p.act, [&](auto tag) {
-                constexpr int kAct = decltype(tag)::value;
+              } else {
 #pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  v[j] = kGated ? gate_act<kAct>(v[j]) * __uint_as_float(ru[j]) : gate_act<kAct>(v[j]);
-              });
-              tile_put<OutT>(my_gen + buf * kTile, lane, v);
-              tile_flush<OutT>(&q.out[0], q.out_ptr[0], q.out_ld[0], q.tma_out[0], my_gen + buf * kTile,
-                               my_addr + buf * kTile, m0, col0, 0, q.m, q.n, lane);
+                for (int j = 0; j < 16; ++j) to[j] = src != nullptr && col0 + j < q.n ? __ldg(src + col0 + j) : 0.0f;
+              }
+            };
+            const int n0 = w.nt * (kGated ? block_n >> 1 : block_n) + g * width;
+            for (int c = group; c < width / kCols; c += kStep) {
+              const int col0 = n0 + c * kCols;
+              if (col0 >= q.n) break;
+              tile_free();
+#pragma unroll
+              for (int h = 0; h < kCols / 16; ++h) {
+                uint32_t r[16], ru[16];
+                load16(c * kCols + h * 16, r);
+                if constexpr (kGated) load16(half_n + c * kCols + h * 16, ru);
+                float cs[16], more[16];                      // scales; the other scales, or the bias
+                columns16(p.col_scale, col0 + h * 16, cs);
+                columns16(kGated ? p.col_scale2 : p.bias, col0 + h * 16, more);
+                ptx::tmem_ld_wait();
+                float v[16];
+                for_act(p.act, [&](auto tag) {
+                  constexpr int kAct = decltype(tag)::value;
+#pragma unroll
+                  for (int j = 0; j < 16; ++j) {
+                    if constexpr (kGated)
+                      v[j] = gate_act<kAct>(value(r[j]) * (rs * cs[j])) * (value(ru[j]) * (rs * more[j]));
+                    else
+                      v[j] = gate_act<kAct>(fmaf(value(r[j]), rs * cs[j], more[j]));
+                  }
+                });
+                tile_put16<OutT>(my_gen, lane, h, v);
+              }
+              flush(0, col0);
             }
           }
         }
@@ -774,7 +813,9 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
 
 // Shared memory beside the stages.
 inline size_t narrow_fixed_bytes(int epi) {
-  return 1024 + kNarrowEpiWarps * static_cast<size_t>(epi == kEpiGatedGrad ? 12288 : 4096) + kNarrowBarBytes;
+  const int staging = epi == kEpiGatedGrad ? kEpiWarps<kEpiGatedGrad> * kStagingWarp<kEpiGatedGrad>
+                                           : kEpiWarps<kEpiStore> * kStagingWarp<kEpiStore>;
+  return 1024 + static_cast<size_t>(staging) + kNarrowBarBytes;
 }
 
 // ------------------------------------------------------------- K-split reduction ---

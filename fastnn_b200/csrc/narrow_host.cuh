@@ -355,7 +355,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   const uint32_t half_n = p.mma_n / 2;
   DType out, f32;
   if (!dtype_of(l.out_code, &out) || !dtype_of(FASTNN_B200_F32, &f32)) return -1;
-  const MapSwizzle out_swz = out.bytes == 4 ? kSwz128 : kSwz64;
+  const uint32_t out_cols = 64 / out.bytes;           // a staging tile: 32 rows of 64 bytes
   bool ok = true;
   long long units = 0;
   for (int i = 0; i < count; ++i) {
@@ -369,6 +369,12 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
     d.first_unit = static_cast<int>(units);
     units += 1ll * d.tiles_m * d.tiles_n * d.split_k;
     if (units > 0x3fffffffll) return -1;
+    d.full_groups = d.tiles_m / kNarrowGroupM;
+    const int last = d.tiles_m - d.full_groups * kNarrowGroupM;
+    d.by_split = fast_div(d.split_k);
+    d.by_group = fast_div(kNarrowGroupM * d.tiles_n);
+    d.by_rows = fast_div(kNarrowGroupM);
+    d.by_last = fast_div(last > 0 ? last : 1);
     d.a_mn = q.a_mn ? 1 : 0; d.b_mn = q.b_mn ? 1 : 0;
     const MapSwizzle mn_swz = l.in.kind == kKindTf32 ? kSwz128Atom32 : kSwz128;
     for (int j = 0; j < 2; ++j) {
@@ -382,12 +388,12 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
                                  q.b_mn ? mn_swz : kSwz128);
       if (q.aux[j] != nullptr)
         ok = ok && encode_narrow(&d.aux[j], out, q.aux[j], q.n, q.m, 1, q.aux_ld * out.bytes,
-                                 q.aux_ld * out.bytes * q.m, 32, 32, out_swz);
+                                 q.aux_ld * out.bytes * q.m, out_cols, 32, kSwz64);
     }
     if (q.split > 1) {
       const long long ld = partial_ld(q);
       d.tma_out[0] = 1;
-      ok = ok && encode_narrow(&d.out[0], f32, q.partials, q.n, q.m, q.split, ld * 4, ld * 4 * q.m, 32, 32, kSwz128);
+      ok = ok && encode_narrow(&d.out[0], f32, q.partials, q.n, q.m, q.split, ld * 4, ld * 4 * q.m, 16, 32, kSwz64);
     } else {
       for (int j = 0; j < 3; ++j) {
         if (q.out[j] == nullptr) continue;
@@ -396,7 +402,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
         d.tma_out[j] = rows_addressable(q.out[j], q.out_ld[j], out.bytes) ? 1 : 0;
         if (d.tma_out[j])
           ok = ok && encode_narrow(&d.out[j], out, q.out[j], q.n, q.m, 1, q.out_ld[j] * out.bytes,
-                                   q.out_ld[j] * out.bytes * q.m, 32, 32, out_swz);
+                                   q.out_ld[j] * out.bytes * q.m, out_cols, 32, kSwz64);
       }
     }
   }
@@ -407,7 +413,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   const size_t fixed = narrow_fixed_bytes(l.epi);
   const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
   p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;
-  p.group_m = 8;
+  p.group_m = kNarrowGroupM;
   p.act = l.act;
   p.is_bf16 = l.in.code == FASTNN_B200_BF16 ? 1 : 0;
   p.row_scale = l.row_scale; p.col_scale = l.col_scale; p.col_scale2 = l.col_scale2; p.bias = l.bias;
@@ -417,7 +423,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   const int clusters = p.total_units < st->max_clusters ? p.total_units : st->max_clusters;
   const NarrowKernel<N> k = pair_kernel<N>(l.in.kind, l.epi, l.out_code);
   if (k == nullptr || clusters < 1) return -1;
-  if (launch_dependent(k, 2 * clusters, kNarrowThreads, fixed + p.num_stages * stage, stream, p) != 0) return -1;
+  if (launch_dependent(k, 2 * clusters, l.epi == kEpiGatedGrad ? kNarrowThreads<kEpiGatedGrad> : kNarrowThreads<kEpiStore>, fixed + p.num_stages * stage, stream, p) != 0) return -1;
   t_last = LastCall{12, plan.block_n, t[0].split, 2 * clusters};
 
   NarrowReduceParams r;
