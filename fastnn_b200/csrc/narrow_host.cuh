@@ -184,7 +184,7 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
       const int len = ceil_div(max_kb, parts);                  // k-blocks of a unit, at most
       if (parts > 1 && len < 4) break;
       if (may_split && want_split > 0 && parts != want_split) continue;
-      double most = 0.0, reduce = 0.0;
+      double most = 0.0, partial = 0.0;
       double unit[fnn::kNarrowMaxProblems];
       long long units[fnn::kNarrowMaxProblems];
       for (int i = 0; i < count; ++i) {
@@ -192,7 +192,7 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
         const double main = ceil_div(t[i].num_kb, split) * per_kb;
         unit[i] = (main > drain ? main : drain) + 300.0 + (bn == 512 ? 0.3 * drain : 0.0);
         units[i] = 1ll * ceil_div(t[i].m, 256) * ceil_div(t[i].n, epi_gated(epi) ? bn / 2 : bn) * split;
-        if (split > 1) reduce += 8.0 * split * t[i].m * t[i].n / 3400.0 / 2.0;   // written and read, mostly in L2
+        if (split > 1) partial += 4.0 * split * t[i].m * t[i].n;
       }
       // units of problem i on pair c: those u in [first, first + units) with u % clusters == c
       for (int c = 0; c < clusters; ++c) {
@@ -205,7 +205,8 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
         }
         if (sum > most) most = sum;
       }
-      if (reduce > 0.0) reduce += 5000.0;
+      // partial sums are written and read once, at a third of the cost while they stay in L2
+      const double reduce = partial > 0.0 ? 5000.0 + 2.0 * partial / (partial < 48e6 ? 10200.0 : 3400.0) : 0.0;
       const double cost = most + drain + reduce;
       if (cost < best) { best = cost; best_bn = bn; best_len = len; }
     }
