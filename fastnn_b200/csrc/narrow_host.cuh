@@ -452,15 +452,27 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   return 0;
 }
 
-// Few tokens take the form with the weights on the M side; set_policy(4) keeps CTA pairs.
-bool use_skinny(int tokens) { return tokens <= fnn::kSkinnyMaxTokens && t_policy.policy != 4; }
+// Few tokens take the form with the weights on the M side, and so do a few hundred while its tiles fit the
+// machine once: CTA pairs then have fewer tiles than SMs and cannot cut K under a gated epilogue (200
+// tokens, 1024 x 1024 block: 12 against 18 us; 2048 x 2048: 20 / 26; 4096 x 16384, 512 tiles: 120 / 97).
+// set_policy(3) and (4) force it and CTA pairs.
+bool use_skinny(int tokens, int n, int epi) {
+  if (t_policy.policy == 3 || t_policy.policy == 4) return t_policy.policy == 3;
+  if (tokens <= fnn::kSkinnyTokens) return true;
+  return tokens <= 512 && 1ll * ceil_div(n, epi_gated(epi) ? 64 : 128) * ceil_div(tokens, fnn::kSkinnyTokens) <= 256;
+}
 
-// K slices of a row tile (the CTAs of one cluster).
-int skinny_split(int tiles, int num_kb) {
+// K slices of a row tile, the CTAs of one cluster: enough for most of the SMs to have a CTA, twice that
+// while every slice keeps eight k-blocks (bytes in flight against meeting costs: 8-bit 4096 x 4096, 1
+// token: 13.1 / 9.1 / 7.2 / 7.5 us with 1 / 2 / 4 / 8 slices), and no more than four for many tokens,
+// whose partial sums cross the cluster (1024 x 1024 block, 128 tokens: 11.7 us with four, 13.9 with eight).
+int skinny_split(long long tiles, int num_kb, int n_mma) {
   int want = t_policy.split_k;
   if (want == 0) {
     want = 1;
-    while (want < 8 && tiles * want < 256) want *= 2;
+    while (want < 8 && tiles * want < 120) want *= 2;
+    if (want < 8 && num_kb / want >= 16 && tiles * want * 2 <= 296) want *= 2;
+    if (n_mma > 64 && want > 4) want = 4;
   }
   int split = 8;
   while (split > 1 && (split > want || num_kb < 2 * split)) split /= 2;
@@ -476,10 +488,12 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
   const int kblock = 128 / l.in.bytes;
   const int tile_rows = two ? 64 : 128;
   p.tokens = t.m; p.n = t.n;
-  p.n_mma = ceil_div(t.m, 16) * 16;
+  p.t_tiles = ceil_div(t.m, kSkinnyTokens);
+  p.n_mma = ceil_div(ceil_div(t.m, p.t_tiles), 16) * 16;
+  p.t_tiles = ceil_div(t.m, p.n_mma);
   p.num_kb = ceil_div(t.k, kblock);
   const int tiles = ceil_div(t.n, tile_rows);
-  p.split = skinny_split(tiles, p.num_kb);
+  p.split = skinny_split(1ll * tiles * p.t_tiles, p.num_kb, p.n_mma);
   bool ok = encode_narrow(&p.x, l.in, t.a[0].p, t.a[0].cols, t.a[0].rows, 1, t.a[0].ld * l.in.bytes,
                           t.a[0].ld * l.in.bytes * t.a[0].rows, kblock, p.n_mma, kSwz128);
   for (int j = 0; j < (two ? 2 : 1); ++j)
@@ -517,12 +531,13 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
   if (smem < floor_bytes) smem = floor_bytes;
   SkinnyKernel k = skinny_kernel(l.in.kind, l.epi, l.out_code);
   if (k == nullptr || smem > kSkinnySmem) return -1;
-  const long long grid = 1ll * tiles * p.split;
+  const long long grid = 1ll * tiles * p.t_tiles * p.split;
   if (grid > 0x7fffffffll) return -1;
   cudaLaunchConfig_t cfg;
   std::memset(&cfg, 0, sizeof(cfg));
   cfg.gridDim = dim3(static_cast<unsigned>(grid), 1, 1);
-  cfg.blockDim = dim3(kSkinnyThreads, 1, 1);
+  const int epi_warps = p.n_mma <= 16 ? 4 : (p.n_mma <= 64 ? 8 : kSkinnyMaxEpiWarps);
+  cfg.blockDim = dim3(32 * (2 + epi_warps), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attrs[2];
@@ -578,26 +593,24 @@ int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cu
   t2.b[0] = wd; t2.b[1] = Mat{nullptr, 0, 0, 0};
   t2.m = a.rows; t2.n = a.d; t2.k = a.f;
   t2.out[0] = a.y; t2.out_ld[0] = a.d;
-  NarrowLaunch l{a.t, a.t.code, fnn::kEpiGated, a.act};
-  if (use_skinny(a.rows)) {
-    if (dry) return 0;
-    if (!ws.fits()) return -1;
-    if (pk.launch(s) != 0 || launch_skinny(st, l, t1, false, s) != 0) return -1;
-    l.epi = fnn::kEpiStore;
-    // Wd may be read early: the launch ahead writes only h, gate and up, and has itself waited for
-    // whatever came before it
-    return launch_skinny(st, l, t2, true, s);
-  }
   const int cl = clusters_of(st);
-  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGated, false);
-  const NarrowPlan p2 = plan_narrow(&t2, 1, kblock, cl, fnn::kEpiStore, true);
-  reserve_partials(ws, &t2, 1);
+  const bool skinny1 = use_skinny(a.rows, a.f, fnn::kEpiGated);
+  const bool skinny2 = use_skinny(a.rows, a.d, fnn::kEpiStore);
+  NarrowPlan p1{0}, p2{0};
+  if (!skinny1) p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGated, false);
+  if (!skinny2) {
+    p2 = plan_narrow(&t2, 1, kblock, cl, fnn::kEpiStore, true);
+    reserve_partials(ws, &t2, 1);
+  }
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
-  if (launch_pair<1>(st, l, &t1, 1, p1, s) != 0) return -1;
+  NarrowLaunch l{a.t, a.t.code, fnn::kEpiGated, a.act};
+  if ((skinny1 ? launch_skinny(st, l, t1, false, s) : launch_pair<1>(st, l, &t1, 1, p1, s)) != 0) return -1;
   l.epi = fnn::kEpiStore;
-  return launch_pair<1>(st, l, &t2, 1, p2, s);
+  // Wd may be read early: the launch ahead writes only h, gate and up, and lets this one start only after
+  // it has itself seen everything before it finish
+  return skinny2 ? launch_skinny(st, l, t2, true, s) : launch_pair<1>(st, l, &t2, 1, p2, s);
 }
 
 int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cudaStream_t s) {
@@ -695,7 +708,7 @@ int int8_product(DeviceState* st, const Int8Args& a, Carver& ws, bool pack_all, 
   if (pk.launch(s) != 0) return -1;
   NarrowLaunch l{kInt8, a.out_code, a.gated ? fnn::kEpiScaledGated : fnn::kEpiScaled, a.act};
   l.row_scale = a.xs; l.col_scale = a.ws; l.col_scale2 = a.ws2; l.bias = a.bias;
-  if (use_skinny(a.rows)) return launch_skinny(st, l, t, false, s);
+  if (use_skinny(a.rows, a.n, l.epi)) return launch_skinny(st, l, t, false, s);
   const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), l.epi, false);
   return launch_pair<1>(st, l, &t, 1, p, s);
 }

@@ -1,9 +1,10 @@
 // The same products for few tokens (decoding): the weight's rows on the tensor core's M side.
 //
-//   out[t, r] = epilogue( sum_k x[t, k] * W[r, k] )        t < tokens <= 128
+//   out[t, r] = epilogue( sum_k x[t, k] * W[r, k] )
 //
 // With up to 128 tokens the time is that of reading the weights once, so the form is chosen for bytes in
-// flight and for even shares of them.  A CTA takes 128 rows of W (a gated product: 64 rows of the gate's
+// flight and for even shares of them; a few hundred are cut into equal tiles of at most 128, whose CTAs
+// stand side by side in the grid and meet the weights in L2.  A CTA takes 128 rows of W (a gated product: 64 rows of the gate's
 // weight and the same 64 of the up projection's) and one slice of K, and streams them through a ring of
 // TMA stages; the tokens are the MMA's N (rounded up to 16, rows past the last one read as zero), so one
 // tcgen05.mma per 32 bytes of K covers all of them and the tensor core is never what is waited for.
@@ -17,8 +18,12 @@
 
 namespace fnn {
 
-constexpr int kSkinnyMaxTokens = 128;
-constexpr int kSkinnyThreads = 192;                 // producer, MMA issuer, four warps that drain the accumulator
+constexpr int kSkinnyTokens = 128;                  // tokens of a tile, at most
+// Producer, MMA issuer, and four to sixteen warps that drain the accumulator and apply the epilogue: at
+// 128 tokens and a short K the epilogue is most of a CTA's life, with a few tokens more warps only start
+// and meet later.
+constexpr int kSkinnyMaxEpiWarps = 16;
+constexpr int kSkinnyMaxThreads = 32 * (2 + kSkinnyMaxEpiWarps);
 constexpr int kSkinnyMaxStages = 8;
 constexpr int kSkinnyBarBytes = 256;
 
@@ -28,7 +33,8 @@ struct SkinnyParams {
   long long out_ld[3];
   int vec_out[3];            // rows may be written four columns at a time
   int tokens, n;             // n: columns of one output
-  int n_mma;                 // tokens rounded up to 16
+  int t_tiles;               // token tiles
+  int n_mma;                 // tokens of a tile, a multiple of 16
   int num_kb, split, num_stages, tmem_cols;
   int early_w;               // the weights may be read before the kernel ahead of this one has finished
   int act, is_bf16;
@@ -59,11 +65,18 @@ __device__ __forceinline__ void mma_narrow_1cta(uint32_t tmem_d, uint64_t desc_a
 }
 }  // namespace ptx
 
-// Four sums over the slices of one token's consecutive rows.
+// Four sums over the slices of one token's consecutive rows, in slice order.
 template <int kKind>
-__device__ __forceinline__ void skinny_sum(uint32_t local, int split, float (&v)[4]) {
-  if constexpr (kKind == kKindI8) {
+__device__ __forceinline__ void skinny_sum(const uint8_t* own, uint32_t local, int split, float (&v)[4]) {
+  if (split == 1) {
+    const uint4 t = *reinterpret_cast<const uint4*>(own);
+    const uint32_t w[4] = {t.x, t.y, t.z, t.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      v[j] = kKind == kKindI8 ? static_cast<float>(static_cast<int>(w[j])) : __uint_as_float(w[j]);
+  } else if constexpr (kKind == kKindI8) {
     int s[4] = {0, 0, 0, 0};
+#pragma unroll 4
     for (int r = 0; r < split; ++r) {
       const float4 t = ptx::ld_shared_cluster_f4(ptx::mapa_shared(local, static_cast<uint32_t>(r)));
       s[0] += __float_as_int(t.x); s[1] += __float_as_int(t.y); s[2] += __float_as_int(t.z); s[3] += __float_as_int(t.w);
@@ -73,6 +86,7 @@ __device__ __forceinline__ void skinny_sum(uint32_t local, int split, float (&v)
   } else {
 #pragma unroll
     for (int j = 0; j < 4; ++j) v[j] = 0.0f;
+#pragma unroll 4
     for (int r = 0; r < split; ++r) {
       const float4 t = ptx::ld_shared_cluster_f4(ptx::mapa_shared(local, static_cast<uint32_t>(r)));
       v[0] += t.x; v[1] += t.y; v[2] += t.z; v[3] += t.w;
@@ -94,7 +108,7 @@ __device__ __forceinline__ void skinny_put(void* out, long long ld, int vec, int
 }
 
 template <int kKind, int kEpi, typename OutT>
-__global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __grid_constant__ SkinnyParams p) {
+__global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(const __grid_constant__ SkinnyParams p) {
   using K = NarrowKind<kKind>;
   constexpr bool kTwo = kEpi == kEpiGated || kEpi == kEpiScaledGated;
   constexpr int kRows = kTwo ? 64 : 128;              // output columns of a tile
@@ -103,6 +117,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
   uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
+  const int epi_warps = static_cast<int>(blockDim.x >> 5) - 2;
   const uint32_t x_bytes = static_cast<uint32_t>(p.n_mma) * 128u;
   const uint32_t stage_bytes = kNarrowABytes + x_bytes;       // x_bytes is a multiple of 2048
   const uint32_t bar_base = smem_base + p.num_stages * stage_bytes;
@@ -115,8 +130,9 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
   volatile int* abort_flag = reinterpret_cast<volatile int*>(bar_gen + 140);
 
   const int slice = static_cast<int>(blockIdx.x) % p.split;   // = rank in the cluster
-  const int tile = static_cast<int>(blockIdx.x) / p.split;
-  const int r0 = tile * kRows;
+  const int unit = static_cast<int>(blockIdx.x) / p.split;
+  const int r0 = unit / p.t_tiles * kRows;
+  const int t0 = unit % p.t_tiles * p.n_mma;
   const int kb0 = static_cast<int>(static_cast<long long>(slice) * p.num_kb / p.split);
   const int kb1 = static_cast<int>(static_cast<long long>(slice + 1) * p.num_kb / p.split);
 
@@ -132,7 +148,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
     }
   };
   auto load_x = [&](int kb, int s) {
-    ptx::tma_load_3d(smem_base + s * stage_bytes + kNarrowABytes, &p.x, full_bar(s), kb * K::kBlock, 0, 0);
+    ptx::tma_load_3d(smem_base + s * stage_bytes + kNarrowABytes, &p.x, full_bar(s), kb * K::kBlock, t0, 0);
   };
 
   int pre = 0;
@@ -211,7 +227,7 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
       const int q = warp & 3;
       const uint32_t taddr = tmem_base + (static_cast<uint32_t>(q * 32) << 16);
       uint32_t* part = reinterpret_cast<uint32_t*>(smem_gen) + q * 32 + lane;
-      for (int c = 0; c < p.n_mma; c += 16) {
+      for (int c = ((warp - 2) >> 2) * 16; c < p.n_mma; c += 4 * epi_warps) {
         uint32_t r[16];
         ptx::tmem_ld_32x16(taddr + c, r);
         ptx::tmem_ld_wait();
@@ -227,22 +243,31 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
   __syncwarp();
   ptx::cluster_arrive_release();
   ptx::cluster_wait_acquire();
-  if (!*abort_flag) {
+  if (!*abort_flag && warp >= 2) {
+    // A thread keeps its four columns and walks over the tokens; the cluster's CTAs take tokens in turn.
     constexpr int kQuads = kRows / 4;
-    const int total = p.tokens * kQuads;
-    for (int i = slice * kSkinnyThreads + static_cast<int>(threadIdx.x); i < total; i += p.split * kSkinnyThreads) {
-      const int t = i / kQuads;
-      const int r = (i - t * kQuads) * 4;
-      const int c = r0 + r;
-      if (c >= p.n) continue;
-      const uint32_t local = smem_base + static_cast<uint32_t>(t * 128 + r) * 4u;
-      float v[4];
-      skinny_sum<kKind>(local, p.split, v);
-      if constexpr (kEpi == kEpiStore) {
-        skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
-      } else if constexpr (kEpi == kEpiGated) {
-        float u[4];
-        skinny_sum<kKind>(local + 64 * 4, p.split, u);
+    const int at_once = 32 * epi_warps / kQuads;               // tokens one CTA covers per step
+    const int tid = static_cast<int>(threadIdx.x) - 64;
+    const int r = tid % kQuads * 4;
+    const int c = r0 + r;
+    const int tokens = c < p.n ? min(p.tokens - t0, p.n_mma) : 0;
+    float cs[4], more[4];
+    if constexpr (kEpi == kEpiScaled || kEpi == kEpiScaledGated) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool in = c + j < p.n;
+        cs[j] = in ? __ldg(p.col_scale + c + j) : 0.0f;
+        if constexpr (kEpi == kEpiScaledGated) more[j] = in ? __ldg(p.col_scale2 + c + j) : 0.0f;
+        else more[j] = in && p.bias != nullptr ? __ldg(p.bias + c + j) : 0.0f;
+      }
+    }
+    for (int tl = slice * at_once + tid / kQuads; tl < tokens; tl += p.split * at_once) {
+      const int t = t0 + tl;
+      const uint32_t off = static_cast<uint32_t>(tl * 128 + r) * 4u;
+      float v[4], u[4];
+      skinny_sum<kKind>(smem_gen + off, smem_base + off, p.split, v);
+      if constexpr (kTwo) skinny_sum<kKind>(smem_gen + off + 256, smem_base + off + 256, p.split, u);
+      if constexpr (kEpi == kEpiGated) {
         if (p.out[1] != nullptr) {
           skinny_put<OutT>(p.out[1], p.out_ld[1], p.vec_out[1], t, c, p.n, v);
           skinny_put<OutT>(p.out[2], p.out_ld[2], p.vec_out[2], t, c, p.n, u);
@@ -252,18 +277,8 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = gate_act<kAct>(v[j]) * u[j];
         });
-        skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
-      } else {
+      } else if constexpr (kEpi != kEpiStore) {
         const float rs = __ldg(p.row_scale + t);
-        float cs[4], more[4], u[4];
-        if constexpr (kEpi == kEpiScaledGated) skinny_sum<kKind>(local + 64 * 4, p.split, u);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool in = c + j < p.n;
-          cs[j] = in ? __ldg(p.col_scale + c + j) : 0.0f;
-          if constexpr (kEpi == kEpiScaledGated) more[j] = in ? __ldg(p.col_scale2 + c + j) : 0.0f;
-          else more[j] = in && p.bias != nullptr ? __ldg(p.bias + c + j) : 0.0f;
-        }
         for_act(p.act, [&](auto tag) {
           constexpr int kAct = decltype(tag)::value;
 #pragma unroll
@@ -274,8 +289,8 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
               v[j] = gate_act<kAct>(fmaf(v[j], rs * cs[j], more[j]));
           }
         });
-        skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
       }
+      skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
     }
   }
   __syncwarp();
@@ -283,8 +298,8 @@ __global__ void __launch_bounds__(kSkinnyThreads) narrow_skinny_kernel(const __g
   ptx::cluster_wait_acquire();
 
   if (*abort_flag) {
-    const long long t0 = clock64();
-    while (clock64() - t0 < 2000000) { }
+    const long long began = clock64();
+    while (clock64() - began < 2000000) { }
   }
   ptx::tc_fence_before_sync();
   __syncthreads();
