@@ -736,7 +736,7 @@ int quantize_launch(const void* x, long long ld, int8_t* q, float* scale, int ro
 extern "C" size_t fastnn_b200_gated_ffn_workspace(int dtype, int rows, int d_model, int d_ff, int backward,
                                                   int unaligned) {
   DType t;
-  if (!dtype_of(dtype, &t) || !ffn_sizes_ok(rows, d_model, d_ff)) return 0;
+  if (!dtype_of(dtype, &t) || !ffn_sizes_ok(rows, d_model, d_ff) || rows == 0) return 0;
   Carver ws{nullptr, 0, true};
   const FfnArgs a = ffn_shape(t, rows, d_model, d_ff);
   if (backward) ffn_backward(current_state(), a, ws, unaligned != 0, nullptr);
@@ -833,7 +833,7 @@ Int8Args int8_shape(int rows, int k, int n, bool gated) {
 }  // namespace
 
 extern "C" size_t fastnn_b200_int8_workspace(int rows, int in_features, int out_features, int gated, int unaligned) {
-  if (rows < 0 || in_features < 1 || out_features < 1) return 0;
+  if (rows < 1 || in_features < 1 || out_features < 1) return 0;
   Carver ws{nullptr, 0, true};
   int8_product(current_state(), int8_shape(rows, in_features, out_features, gated != 0), ws, unaligned != 0, nullptr);
   return ws.used;
