@@ -85,7 +85,9 @@ struct NarrowProblem {
   int m, n;                    // n: columns of ONE output
   int tiles_m, tiles_n;
   int num_kb, num_kb1;         // 128-byte k-blocks in all, and those of the first operand pair
-  int split_k, kb_per_split;   // split_k > 1: partial sums, FP32, one [m, n] block per slice in out[0]
+  int full_tiles;              // tiles done whole; the others in split_k slices of K, whose FP32 sums go to
+  int split_k, kb_per_split;   // partial: one 256 x block_n block for each (tile, slice), stacked
+  CUtensorMap partial;
   int first_unit;
   int full_groups;             // rasterisation groups of group_m tile rows
   FastDiv by_split, by_group, by_rows, by_last;   // K slices; tiles of a full group; tile rows of a group, of the last
@@ -337,7 +339,7 @@ __device__ __forceinline__ bool narrow_wait(uint32_t bar, uint32_t parity, volat
 }
 
 struct NarrowUnit {
-  int pr, s, mt, nt, kb0, kb1;
+  int pr, slot, mt, nt, kb0, kb1;      // slot: block of partial sums, -1 for a whole tile
 };
 template <int kProblems>
 __device__ __forceinline__ NarrowUnit narrow_unit(const NarrowParams<kProblems>& p, int u) {
@@ -348,15 +350,23 @@ __device__ __forceinline__ NarrowUnit narrow_unit(const NarrowParams<kProblems>&
   const NarrowProblem& q = p.pr[i];
   int t = u - q.first_unit;
   w.pr = i;
-  const int tile = div_by(t, q.by_split);
-  w.s = t - tile * q.split_k;
+  int tile = t;
+  w.slot = -1;
+  w.kb0 = 0;
+  w.kb1 = q.num_kb;
+  if (t >= q.full_tiles) {
+    w.slot = t - q.full_tiles;
+    const int k = div_by(w.slot, q.by_split);
+    const int slice = w.slot - k * q.split_k;
+    tile = q.full_tiles + k;
+    w.kb0 = slice * q.kb_per_split;
+    w.kb1 = min(q.num_kb, w.kb0 + q.kb_per_split);
+  }
   const int g = div_by(tile, q.by_group);
   const int r = tile - g * static_cast<int>(q.by_group.d);
   const FastDiv& rows = g < q.full_groups ? q.by_rows : q.by_last;
   w.nt = div_by(r, rows);
   w.mt = g * p.group_m + r - w.nt * static_cast<int>(rows.d);
-  w.kb0 = w.s * q.kb_per_split;
-  w.kb1 = min(q.num_kb, w.kb0 + q.kb_per_split);
   return w;
 }
 
@@ -573,7 +583,6 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
       const NarrowProblem& q = p.pr[w.pr];
       const int m0 = w.mt * 256 + static_cast<int>(rank) * 128 + q4 * 32;
       const int row = m0 + lane;
-      const bool raw = q.split_k > 1;
       const bool rows_live = m0 < q.m;                       // warp-uniform
       for (int g = 0; g < groups && ok; ++g) {
         ok = narrow_wait(tfull_bar(slot), slot_phase, abort_flag, p, kStatusEpilogueTimeout);
@@ -596,7 +605,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
         if (rows_live) {
           if constexpr (kEpi == kEpiStore) {
             const int n0 = w.nt * block_n + g * p.mma_n;
-            if (raw) {                                       // FP32 partial sums of one K slice
+            if (w.slot >= 0) {                               // FP32 partial sums of one K slice
               for (int c = group; c < p.mma_n / 16; c += kStep) {
                 const int col0 = n0 + c * 16;
                 if (col0 >= q.n) break;
@@ -611,7 +620,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
                 ptx::fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) {
-                  ptx::tma_store_3d(&q.out[0], my_addr, col0, m0, w.s);
+                  ptx::tma_store_3d(&q.partial, my_addr, g * p.mma_n + c * 16, w.slot * 256 + (m0 - w.mt * 256), 0);
                   ptx::tma_store_commit();
                 }
               }
@@ -819,18 +828,19 @@ inline size_t narrow_fixed_bytes(int epi) {
 }
 
 // ------------------------------------------------------------- K-split reduction ---
-// Partial products of up to four problems of one launch, added in slice order and rounded once.
+// The partial sums of up to four problems' split tiles, added in slice order and rounded once.
 struct NarrowReduceItem {
-  const float* partials;       // [slices][rows][ld]
+  const float* partials;       // [tile - first_tile][slice][256][block_n]
   void* out;                   // [rows, cols], row stride out_ld
-  long long ld, slice, out_ld;
-  int rows, cols, slices, first_block;
+  long long out_ld;
+  int rows, cols, slices, first_tile, tiles_m, tiles_n, first_block;
+  int vec;                     // rows of out may be written four columns at a time
 };
 struct NarrowReduceParams {
   NarrowReduceItem it[kNarrowMaxProblems];
-  int count;
+  int count, block_n, group_m;
 };
-constexpr int kReduceCols = 4;                     // columns per thread
+constexpr int kReduceRows = 4;                     // rows of a tile one block adds up
 template <typename T>
 __global__ void __launch_bounds__(256) narrow_reduce_kernel(const __grid_constant__ NarrowReduceParams p) {
   ptx::grid_dep_wait();
@@ -838,22 +848,39 @@ __global__ void __launch_bounds__(256) narrow_reduce_kernel(const __grid_constan
   int i = 0;
   while (i + 1 < p.count && static_cast<int>(blockIdx.x) >= p.it[i + 1].first_block) ++i;
   const NarrowReduceItem& q = p.it[i];
-  const int per_row = (q.cols + kReduceCols - 1) / kReduceCols;
-  const long long idx = static_cast<long long>(blockIdx.x - q.first_block) * 256 + threadIdx.x;
-  const long long r = idx / per_row;
-  if (r >= q.rows) return;
-  const int c = static_cast<int>(idx - r * per_row) * kReduceCols;
-  const float* src = q.partials + r * q.ld + c;    // ld is a multiple of 4: aligned, and the padding is readable
-  float4 s = *reinterpret_cast<const float4*>(src);
-  for (int k = 1; k < q.slices; ++k) {
-    const float4 t = *reinterpret_cast<const float4*>(src + k * q.slice);
-    s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
-  }
-  T* dst = static_cast<T*>(q.out) + r * q.out_ld + c;
-  const float v[4] = {s.x, s.y, s.z, s.w};
+  const int b = static_cast<int>(blockIdx.x) - q.first_block;
+  const int k = b / (256 / kReduceRows);                       // split tile
+  const int tile = q.first_tile + k;
+  // the tile's place, as narrow_unit finds it
+  const int group_sz = p.group_m * q.tiles_n;
+  const int first_m = tile / group_sz * p.group_m;
+  const int gm = min(q.tiles_m - first_m, p.group_m);
+  const int r = tile % group_sz;
+  const int row0 = b % (256 / kReduceRows) * kReduceRows;
+  const int m0 = (first_m + r % gm) * 256 + row0, n0 = r / gm * p.block_n;
+  const int quads = p.block_n >> 2;
+  const float* src = q.partials + (static_cast<long long>(k) * q.slices * 256 + row0) * p.block_n;
+  const long long slice = 256ll * p.block_n;
+  for (int e = threadIdx.x; e < kReduceRows * quads; e += 256) {
+    const int rr = e / quads, c = (e - rr * quads) * 4;
+    if (m0 + rr >= q.rows || n0 + c >= q.cols) continue;
+    const float* at = src + rr * p.block_n + c;
+    float4 s = *reinterpret_cast<const float4*>(at);
+    for (int j = 1; j < q.slices; ++j) {
+      const float4 t = *reinterpret_cast<const float4*>(at + j * slice);
+      s.x += t.x; s.y += t.y; s.z += t.z; s.w += t.w;
+    }
+    const float v[4] = {s.x, s.y, s.z, s.w};
+    T* dst = static_cast<T*>(q.out) + static_cast<long long>(m0 + rr) * q.out_ld + n0 + c;
+    if (q.vec && n0 + c + 4 <= q.cols) {
+      if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = s;
+      else *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]));
+    } else {
 #pragma unroll
-  for (int j = 0; j < 4; ++j)
-    if (c + j < q.cols) dst[j] = static_cast<T>(v[j]);
+      for (int j = 0; j < 4; ++j)
+        if (n0 + c + j < q.cols) dst[j] = static_cast<T>(v[j]);
+    }
+  }
 }
 
 // ------------------------------------------------------------------- row packing ---

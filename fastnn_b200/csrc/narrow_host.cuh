@@ -146,7 +146,7 @@ struct NarrowTask {
   const void* aux[2] = {nullptr, nullptr};     // kEpiGatedGrad: gate and up
   long long aux_ld = 0;
   // plan
-  int split = 1, kb_per_split = 0, num_kb1 = 0, num_kb = 0;
+  int full = 0, split = 1, kb_per_split = 0, num_kb1 = 0, num_kb = 0;   // whole tiles; slices of the others
   float* partials = nullptr;
 };
 
@@ -163,7 +163,11 @@ struct NarrowPlan {
 inline bool epi_gated(int epi) { return epi == fnn::kEpiGated || epi == fnn::kEpiScaledGated; }
 struct PlanChoice {
   int block_n, len;          // len: k-blocks of a unit, at most
+  bool keep_full;            // a problem's whole waves of tiles stay uncut, only its last tiles are split
 };
+inline int tiles_of(const NarrowTask& t, int bn, int epi) {
+  return ceil_div(t.m, 256) * ceil_div(t.n, epi_gated(epi) ? bn / 2 : bn);
+}
 PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int clusters, int epi, bool may_split,
                          int want_bn, int want_split) {
   int max_kb = 1;
@@ -171,6 +175,7 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
     if (t[i].num_kb > max_kb) max_kb = t[i].num_kb;
   double best = 1e300;
   int best_bn = 256, best_len = max_kb;
+  bool best_keep = false;
   // a CTA's half of an MN-major B tile is whole 128-byte chunks of N
   int min_bn = epi_gated(epi) ? 128 : 64;
   for (int i = 0; i < count; ++i)
@@ -184,34 +189,44 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
       const int len = ceil_div(max_kb, parts);                  // k-blocks of a unit, at most
       if (parts > 1 && len < 4) break;
       if (may_split && want_split > 0 && parts != want_split) continue;
-      double most = 0.0, partial = 0.0;
-      double unit[fnn::kNarrowMaxProblems];
-      long long units[fnn::kNarrowMaxProblems];
-      for (int i = 0; i < count; ++i) {
-        const int split = ceil_div(t[i].num_kb, len);
-        const double main = ceil_div(t[i].num_kb, split) * per_kb;
-        unit[i] = (main > drain ? main : drain) + 300.0 + (bn == 512 ? 0.3 * drain : 0.0);
-        units[i] = 1ll * ceil_div(t[i].m, 256) * ceil_div(t[i].n, epi_gated(epi) ? bn / 2 : bn) * split;
-        if (split > 1) partial += 4.0 * split * t[i].m * t[i].n;
-      }
-      // units of problem i on pair c: those u in [first, first + units) with u % clusters == c
-      for (int c = 0; c < clusters; ++c) {
-        double sum = 0.0;
-        long long first = 0;
+      for (int keep = 0; keep < (parts > 1 ? 2 : 1); ++keep) {
+        double most = 0.0, partial = 0.0;
+        double whole[fnn::kNarrowMaxProblems], part[fnn::kNarrowMaxProblems];
+        long long full[fnn::kNarrowMaxProblems], units[fnn::kNarrowMaxProblems];
+        auto clocks = [&](int kb) {
+          const double main = kb * per_kb;
+          return (main > drain ? main : drain) + 300.0 + (bn == 512 ? 0.3 * drain : 0.0);
+        };
         for (int i = 0; i < count; ++i) {
-          const long long lo = (c - first + clusters) % clusters;
-          sum += (lo < units[i] ? (units[i] - lo + clusters - 1) / clusters : 0) * unit[i];
-          first = (first + units[i]) % clusters;
+          const int split = ceil_div(t[i].num_kb, len);
+          const long long tiles = tiles_of(t[i], bn, epi);
+          full[i] = split == 1 ? tiles : (keep ? tiles / clusters * clusters : 0);
+          units[i] = full[i] + (tiles - full[i]) * split;
+          whole[i] = clocks(t[i].num_kb);
+          part[i] = clocks(ceil_div(t[i].num_kb, split));
+          if (split > 1) partial += 4.0 * 256 * bn * (tiles - full[i]) * split;
         }
-        if (sum > most) most = sum;
+        // units go round robin: those u in [first, first + units) with u % clusters == c are pair c's
+        for (int c = 0; c < clusters; ++c) {
+          double sum = 0.0;
+          long long first = 0;
+          for (int i = 0; i < count; ++i) {
+            const long long lo = (c - first + clusters) % clusters;
+            auto below = [&](long long n) { return lo < n ? (n - lo + clusters - 1) / clusters : 0; };
+            const long long mine = below(full[i]);
+            sum += mine * whole[i] + (below(units[i]) - mine) * part[i];
+            first = (first + units[i]) % clusters;
+          }
+          if (sum > most) most = sum;
+        }
+        // partial sums are written and read once, at a third of the cost while they stay in L2
+        const double reduce = partial > 0.0 ? 5000.0 + 2.0 * partial / (partial < 48e6 ? 10200.0 : 3400.0) : 0.0;
+        const double cost = most + drain + reduce;
+        if (cost < best) { best = cost; best_bn = bn; best_len = len; best_keep = keep != 0; }
       }
-      // partial sums are written and read once, at a third of the cost while they stay in L2
-      const double reduce = partial > 0.0 ? 5000.0 + 2.0 * partial / (partial < 48e6 ? 10200.0 : 3400.0) : 0.0;
-      const double cost = most + drain + reduce;
-      if (cost < best) { best = cost; best_bn = bn; best_len = len; }
     }
   }
-  return PlanChoice{best_bn, best_len};
+  return PlanChoice{best_bn, best_len, best_keep};
 }
 
 // The choice walks some ten thousand combinations; programs repeat a handful of shapes, so answers are
@@ -245,20 +260,23 @@ NarrowPlan plan_narrow(NarrowTask* t, int count, int kblock, int clusters, int e
     }
     c = slot.choice;
   }
-  const int best_bn = c.block_n, best_len = c.len;
   for (int i = 0; i < count; ++i) {
-    t[i].split = ceil_div(t[i].num_kb, best_len);
+    const int tiles = tiles_of(t[i], c.block_n, epi);
+    t[i].split = ceil_div(t[i].num_kb, c.len);
     t[i].kb_per_split = ceil_div(t[i].num_kb, t[i].split);
     t[i].split = ceil_div(t[i].num_kb, t[i].kb_per_split);
+    t[i].full = t[i].split == 1 ? tiles : (c.keep_full ? tiles / clusters * clusters : 0);
+    if (t[i].full == tiles) t[i].split = 1;
   }
-  return NarrowPlan{best_bn};
+  return NarrowPlan{c.block_n};
 }
 
-inline long long partial_ld(const NarrowTask& t) { return round_up(t.n, 4); }
-void reserve_partials(Carver& ws, NarrowTask* t, int count) {
+// Room for the partial sums of split tiles (of a launch without a gated epilogue).
+void reserve_partials(Carver& ws, NarrowTask* t, int count, const NarrowPlan& plan) {
   for (int i = 0; i < count; ++i)
     if (t[i].split > 1)
-      t[i].partials = static_cast<float*>(ws.take(sizeof(float) * static_cast<size_t>(partial_ld(t[i])) * t[i].m * t[i].split));
+      t[i].partials = static_cast<float*>(ws.take(sizeof(float) * 256 * static_cast<size_t>(plan.block_n) * t[i].split *
+                                                  (tiles_of(t[i], plan.block_n, fnn::kEpiStore) - t[i].full)));
 }
 
 template <int N>
@@ -357,6 +375,8 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   DType out, f32;
   if (!dtype_of(l.out_code, &out) || !dtype_of(FASTNN_B200_F32, &f32)) return -1;
   const uint32_t out_cols = 64 / out.bytes;           // a staging tile: 32 rows of 64 bytes
+  const int group_m = tunables().group_m >= 1 && tunables().group_m <= 1024 ? tunables().group_m
+                      : (l.in.bytes == 1 ? 2 * kNarrowGroupM : kNarrowGroupM);    // 16 MiB of A rows at K = 4096
   bool ok = true;
   long long units = 0;
   for (int i = 0; i < count; ++i) {
@@ -368,13 +388,15 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
     d.num_kb = q.num_kb; d.num_kb1 = q.num_kb1;
     d.split_k = q.split; d.kb_per_split = q.kb_per_split;
     d.first_unit = static_cast<int>(units);
-    units += 1ll * d.tiles_m * d.tiles_n * d.split_k;
+    const long long tiles = 1ll * d.tiles_m * d.tiles_n;
+    d.full_tiles = q.full;
+    units += q.full + (tiles - q.full) * q.split;
     if (units > 0x3fffffffll) return -1;
-    d.full_groups = d.tiles_m / kNarrowGroupM;
-    const int last = d.tiles_m - d.full_groups * kNarrowGroupM;
+    d.full_groups = d.tiles_m / group_m;
+    const int last = d.tiles_m - d.full_groups * group_m;
     d.by_split = fast_div(d.split_k);
-    d.by_group = fast_div(kNarrowGroupM * d.tiles_n);
-    d.by_rows = fast_div(kNarrowGroupM);
+    d.by_group = fast_div(group_m * d.tiles_n);
+    d.by_rows = fast_div(group_m);
     d.by_last = fast_div(last > 0 ? last : 1);
     d.a_mn = q.a_mn ? 1 : 0; d.b_mn = q.b_mn ? 1 : 0;
     const MapSwizzle mn_swz = l.in.kind == kKindTf32 ? kSwz128Atom32 : kSwz128;
@@ -392,19 +414,18 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
                                  q.aux_ld * out.bytes * q.m, out_cols, 32, kSwz64);
     }
     if (q.split > 1) {
-      const long long ld = partial_ld(q);
-      d.tma_out[0] = 1;
-      ok = ok && encode_narrow(&d.out[0], f32, q.partials, q.n, q.m, q.split, ld * 4, ld * 4 * q.m, 16, 32, kSwz64);
-    } else {
-      for (int j = 0; j < 3; ++j) {
-        if (q.out[j] == nullptr) continue;
-        d.out_ptr[j] = q.out[j];
-        d.out_ld[j] = q.out_ld[j];
-        d.tma_out[j] = rows_addressable(q.out[j], q.out_ld[j], out.bytes) ? 1 : 0;
-        if (d.tma_out[j])
-          ok = ok && encode_narrow(&d.out[j], out, q.out[j], q.n, q.m, 1, q.out_ld[j] * out.bytes,
-                                   q.out_ld[j] * out.bytes * q.m, out_cols, 32, kSwz64);
-      }
+      const uint64_t blocks = static_cast<uint64_t>(tiles - q.full) * q.split;
+      ok = ok && encode_narrow(&d.partial, f32, q.partials, plan.block_n, blocks * 256, 1, plan.block_n * 4ull,
+                               blocks * 256 * plan.block_n * 4ull, 16, 32, kSwz64);
+    }
+    for (int j = 0; j < 3; ++j) {
+      if (q.out[j] == nullptr) continue;
+      d.out_ptr[j] = q.out[j];
+      d.out_ld[j] = q.out_ld[j];
+      d.tma_out[j] = rows_addressable(q.out[j], q.out_ld[j], out.bytes) ? 1 : 0;
+      if (d.tma_out[j])
+        ok = ok && encode_narrow(&d.out[j], out, q.out[j], q.n, q.m, 1, q.out_ld[j] * out.bytes,
+                                 q.out_ld[j] * out.bytes * q.m, out_cols, 32, kSwz64);
     }
   }
   if (!ok) return -1;
@@ -414,7 +435,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   const size_t fixed = narrow_fixed_bytes(l.epi);
   const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
   p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;
-  p.group_m = kNarrowGroupM;
+  p.group_m = group_m;
   p.act = l.act;
   p.is_bf16 = l.in.code == FASTNN_B200_BF16 ? 1 : 0;
   p.row_scale = l.row_scale; p.col_scale = l.col_scale; p.col_scale2 = l.col_scale2; p.bias = l.bias;
@@ -435,13 +456,16 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
     NarrowReduceItem& it = r.it[r.count++];
     it.partials = t[i].partials;
     it.out = t[i].out[0];
-    it.ld = partial_ld(t[i]);
-    it.slice = it.ld * t[i].m;
     it.out_ld = t[i].out_ld[0];
     it.rows = t[i].m; it.cols = t[i].n; it.slices = t[i].split;
+    it.first_tile = t[i].full;
+    it.tiles_m = p.pr[i].tiles_m; it.tiles_n = p.pr[i].tiles_n;
+    it.vec = reinterpret_cast<uintptr_t>(it.out) % (4 * out.bytes) == 0 && it.out_ld % 4 == 0 ? 1 : 0;
     it.first_block = static_cast<int>(blocks);
-    blocks += (1ll * t[i].m * ceil_div(t[i].n, kReduceCols) + 255) / 256;
+    blocks += (1ll * it.tiles_m * it.tiles_n - it.first_tile) * (256 / kReduceRows);
   }
+  r.block_n = plan.block_n;
+  r.group_m = group_m;
   if (blocks > 0) {
     if (blocks > 0x7fffffffll) return -1;
     const unsigned g = static_cast<unsigned>(blocks);
@@ -600,7 +624,7 @@ int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cu
   if (!skinny1) p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGated, false);
   if (!skinny2) {
     p2 = plan_narrow(&t2, 1, kblock, cl, fnn::kEpiStore, true);
-    reserve_partials(ws, &t2, 1);
+    reserve_partials(ws, &t2, 1, p2);
   }
   if (dry) return 0;
   if (!ws.fits()) return -1;
@@ -661,7 +685,7 @@ int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, c
   const int cl = clusters_of(st);
   const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGatedGrad, false);
   const NarrowPlan p2 = plan_narrow(g, 4, kblock, cl, fnn::kEpiStore, true);
-  reserve_partials(ws, g, 4);
+  reserve_partials(ws, g, 4, p2);
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
