@@ -101,6 +101,7 @@ struct NarrowParams {
   int groups;                  // 256-column MMA groups of a tile: 2 for wide tiles
   int mma_n;                   // columns of one group's MMA; a tile has groups * mma_n
   int num_stages, group_m;
+  int kb_per_stage;            // k-blocks of a stage: two where the MMA thread's issue would set the pace
   int act, is_bf16;
   const float* row_scale;
   const float* col_scale;
@@ -389,7 +390,8 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   const int half_n = p.mma_n >> 1;                       // B columns of one MMA group this CTA loads
   const int block_n = groups * p.mma_n;
   const uint32_t half_bytes = static_cast<uint32_t>(half_n) * 128u;
-  const uint32_t stage_bytes = kNarrowABytes + static_cast<uint32_t>(groups) * half_bytes;
+  const uint32_t kb_bytes = kNarrowABytes + static_cast<uint32_t>(groups) * half_bytes;
+  const uint32_t stage_bytes = static_cast<uint32_t>(p.kb_per_stage) * kb_bytes;
   const uint32_t staging_base = smem_base + p.num_stages * stage_bytes;
   constexpr int kWarps = kEpiWarps<kEpi>;
   constexpr int kMmaWarpB = 2 + kWarps;                  // second MMA-issuing warp (wide tiles)
@@ -452,31 +454,34 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
         // a gated tile: this CTA's columns are all gate (leader) or all up (peer) columns of the same outputs
         const int n0 = kTwoB ? w.nt * (block_n >> 1) : w.nt * block_n + static_cast<int>(rank) * half_n;
         const int n_step = kTwoB ? half_n : p.mma_n;     // to the next group's columns
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        for (int kb = w.kb0; kb < w.kb1; kb += p.kb_per_stage) {
           ok = narrow_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, kStatusProducerTimeout);
           if (!ok) break;
           const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0);
-          ptx::mbar_expect_tx_cluster(fb, stage_bytes);
-          const uint32_t sa = smem_base + stage * stage_bytes;
-          const bool second = kb >= q.num_kb1;
-          const int k0 = (second ? kb - q.num_kb1 : kb) * K::kBlock;
-          const CUtensorMap* mA = &q.a[second ? 1 : 0];
-          const CUtensorMap* mB = &q.b[kTwoB ? static_cast<int>(rank) : (second ? 1 : 0)];
-          if (!q.a_mn) {
-            ptx::tma_load_3d_pair(sa, mA, fb, k0, m0, 0, pol);
-          } else {
-#pragma unroll
-            for (int c = 0; c < 128 / static_cast<int>(K::kChunkElems); ++c)
-              ptx::tma_load_3d_pair(sa + c * K::kChunkBytes, mA, fb, m0 + c * K::kChunkElems, k0, 0, pol);
-          }
-          for (int g = 0; g < groups; ++g) {
-            const uint32_t sb = sa + kNarrowABytes + g * half_bytes;
-            const int ng = n0 + g * n_step;
-            if (!q.b_mn) {
-              ptx::tma_load_3d_pair(sb, mB, fb, k0, ng, 0, pol);
+          const int count = min(p.kb_per_stage, w.kb1 - kb);
+          ptx::mbar_expect_tx_cluster(fb, count * kb_bytes);
+          for (int i = 0; i < count; ++i) {
+            const uint32_t sa = smem_base + stage * stage_bytes + i * kb_bytes;
+            const bool second = kb + i >= q.num_kb1;
+            const int k0 = (second ? kb + i - q.num_kb1 : kb + i) * K::kBlock;
+            const CUtensorMap* mA = &q.a[second ? 1 : 0];
+            const CUtensorMap* mB = &q.b[kTwoB ? static_cast<int>(rank) : (second ? 1 : 0)];
+            if (!q.a_mn) {
+              ptx::tma_load_3d_pair(sa, mA, fb, k0, m0, 0, pol);
             } else {
-              for (int c = 0; c < half_n / static_cast<int>(K::kChunkElems); ++c)
-                ptx::tma_load_3d_pair(sb + c * K::kChunkBytes, mB, fb, ng + c * K::kChunkElems, k0, 0, pol);
+#pragma unroll
+              for (int c = 0; c < 128 / static_cast<int>(K::kChunkElems); ++c)
+                ptx::tma_load_3d_pair(sa + c * K::kChunkBytes, mA, fb, m0 + c * K::kChunkElems, k0, 0, pol);
+            }
+            for (int g = 0; g < groups; ++g) {
+              const uint32_t sb = sa + kNarrowABytes + g * half_bytes;
+              const int ng = n0 + g * n_step;
+              if (!q.b_mn) {
+                ptx::tma_load_3d_pair(sb, mB, fb, k0, ng, 0, pol);
+              } else {
+                for (int c = 0; c < half_n / static_cast<int>(K::kChunkElems); ++c)
+                  ptx::tma_load_3d_pair(sb + c * K::kChunkBytes, mB, fb, ng + c * K::kChunkElems, k0, 0, pol);
+              }
             }
           }
           if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
@@ -496,8 +501,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
     const int my_group = warp == 1 ? 0 : 1;
     if (lane == 0 && rank == 0 && my_group < groups) {
       const uint64_t stage_step = stage_bytes >> 4;
-      const uint32_t bar0 = ptx::mapa_shared(bar_base, 0);
-      const uint32_t bar1 = ptx::mapa_shared(bar_base, 1);
+      const uint64_t kb_step = kb_bytes >> 4;
       int stage = 0;
       uint32_t phase = 0;
       int slot = my_group;
@@ -516,23 +520,24 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
         ptx::tc_fence_after_sync();
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(slot * kMaxBlockN);
         uint32_t accumulate = 0u;
-        for (int kb = w.kb0; kb < w.kb1; ++kb) {
+        for (int kb = w.kb0; kb < w.kb1; kb += p.kb_per_stage) {
           ok = narrow_wait(full_bar(stage), phase, abort_flag, p, kStatusMmaTimeout);
           if (!ok) break;
-          const uint64_t da = a_desc0 + stage * stage_step;
-          const uint64_t db = b_desc0 + stage * stage_step;
-          ptx::mma_narrow_2cta<kKind>(tmem_d, da, db, idesc, accumulate);
-          accumulate = 1u;
+          const int count = min(p.kb_per_stage, w.kb1 - kb);
+          uint64_t da = a_desc0 + stage * stage_step;
+          uint64_t db = b_desc0 + stage * stage_step;
+          for (int i = 0; i < count; ++i, da += kb_step, db += kb_step) {
+            ptx::mma_narrow_2cta<kKind>(tmem_d, da, db, idesc, accumulate);
+            accumulate = 1u;
 #pragma unroll
-          for (int ks = 1; ks < 4; ++ks)
-            ptx::mma_narrow_2cta<kKind>(tmem_d, da + ks * a_step, db + ks * b_step, idesc, 1u);
-          ptx::mma_commit_2cta(bar0 + 64u + 8u * stage);    // empty[stage], leader
-          ptx::mma_commit_2cta(bar1 + 64u + 8u * stage);    // empty[stage], peer
+            for (int ks = 1; ks < 4; ++ks)
+              ptx::mma_narrow_2cta<kKind>(tmem_d, da + ks * a_step, db + ks * b_step, idesc, 1u);
+          }
+          ptx::mma_commit_2cta_mask(empty_bar(stage), 3);   // the stage is free, in both CTAs
           if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
         }
         if (!ok) break;
-        ptx::mma_commit_2cta(bar0 + 128u + 8u * slot);      // accumulator full, both CTAs
-        ptx::mma_commit_2cta(bar1 + 128u + 8u * slot);
+        ptx::mma_commit_2cta_mask(tfull_bar(slot), 3);      // the accumulator is complete, in both CTAs
         if (groups == 2) slot_phase ^= 1u;
         else if (++slot == 2) { slot = 0; slot_phase ^= 1u; }
       }

@@ -431,7 +431,10 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   if (!ok) return -1;
   p.count = count;
   p.total_units = static_cast<int>(units);
-  const size_t stage = kNarrowABytes + static_cast<size_t>(p.groups) * half_n * 128;
+  // one thread issues a group's MMAs, and a stage's wait and commit cost it as much as an MMA or two: two
+  // k-blocks a stage, except for wide tiles, whose two threads have twice the clocks for the same work
+  p.kb_per_stage = p.groups == 2 ? 1 : (tunables().kb_per_stage >= 1 && tunables().kb_per_stage <= 4 ? tunables().kb_per_stage : 2);
+  const size_t stage = p.kb_per_stage * (kNarrowABytes + static_cast<size_t>(p.groups) * half_n * 128);
   const size_t fixed = narrow_fixed_bytes(l.epi);
   const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
   p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;

@@ -250,6 +250,14 @@ __device__ __forceinline__ void mma_commit_2cta(uint32_t bar) {
                : "memory");
 }
 
+// One commit that arrives on the barrier at this CTA-relative address in every CTA of `cta_mask`.
+__device__ __forceinline__ void mma_commit_2cta_mask(uint32_t bar, uint16_t cta_mask) {
+  asm volatile(
+      "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+      "h"(cta_mask)
+      : "memory");
+}
+
 // TMEM -> registers: this warp's 32 lanes x 32 consecutive 32-bit columns.
 __device__ __forceinline__ void tmem_ld_32x32(uint32_t taddr, uint32_t (&r)[32]) {
   asm volatile(
