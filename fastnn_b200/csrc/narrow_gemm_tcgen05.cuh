@@ -44,7 +44,7 @@ constexpr int kActSilu = 5;
 template <int kEpi>
 constexpr int kEpiWarps = kEpi == kEpiGatedGrad ? 8 : 16;
 template <int kEpi>
-constexpr int kNarrowThreads = 32 * (kEpiWarps<kEpi> + 3);    // + producer and two MMA issuers
+constexpr int kNarrowThreads = 32 * (kEpiWarps<kEpi> + 4);    // + two producers and two MMA issuers
 constexpr int kNarrowMaxProblems = 4;
 constexpr int kNarrowMaxStages = 8;
 constexpr int kNarrowABytes = 128 * 128;             // 128 rows x 128 bytes of K
@@ -395,6 +395,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   const uint32_t staging_base = smem_base + p.num_stages * stage_bytes;
   constexpr int kWarps = kEpiWarps<kEpi>;
   constexpr int kMmaWarpB = 2 + kWarps;                  // second MMA-issuing warp (wide tiles)
+  constexpr int kLoadWarpB = 3 + kWarps;                 // loads B while warp 0 loads A
   const uint32_t bar_base = staging_base + kWarps * kStagingWarp<kEpi>;
   auto full_bar = [&](int s) { return bar_base + 8u * s; };
   auto empty_bar = [&](int s) { return bar_base + 64u + 8u * s; };
@@ -440,51 +441,59 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
 
-  if (warp == 0) {
-    // ------------------------------------------------------------- producer ---
+  if (warp == 0 || warp == kLoadWarpB) {
+    // ------------------------------------------------------------ producers ---
+    // One thread loads A, another B: one thread's wait, announcement and boxes took 600 to 1000 clocks a
+    // k-block, more than the tensor cores (B with two boxes a group: 985 -> 750).  What a unit's loop
+    // needs is in registers; a k-block is `boxes` boxes of each group, `x_step` apart in the matrix.
+    const bool for_a = warp == 0;
     if (lane == 0) {
       int stage = 0;
       uint32_t phase = 0;
       bool ok = true;
       const uint64_t pol = ptx::make_l2_policy(3);
+      const uint32_t full0 = ptx::mapa_shared(full_bar(0), 0);       // the leader's barriers
+      const int n_step = kTwoB ? half_n : p.mma_n;                   // to the next group's columns
+      const int my_groups = for_a ? 1 : groups;
+      const int stages = p.num_stages, per_stage = p.kb_per_stage;
+      const uint32_t my_base = smem_base + (for_a ? 0u : static_cast<uint32_t>(kNarrowABytes));
+      uint32_t ready = 0;
       for (int u = cluster_id; u < p.total_units && ok; u += num_clusters) {
         const NarrowUnit w = narrow_unit(p, u);
         const NarrowProblem& q = p.pr[w.pr];
-        const int m0 = w.mt * 256 + static_cast<int>(rank) * 128;
         // a gated tile: this CTA's columns are all gate (leader) or all up (peer) columns of the same outputs
-        const int n0 = kTwoB ? w.nt * (block_n >> 1) : w.nt * block_n + static_cast<int>(rank) * half_n;
-        const int n_step = kTwoB ? half_n : p.mma_n;     // to the next group's columns
-        for (int kb = w.kb0; kb < w.kb1; kb += p.kb_per_stage) {
-          ok = narrow_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, kStatusProducerTimeout);
-          if (!ok) break;
-          const uint32_t fb = ptx::mapa_shared(full_bar(stage), 0);
-          const int count = min(p.kb_per_stage, w.kb1 - kb);
-          ptx::mbar_expect_tx_cluster(fb, count * kb_bytes);
-          for (int i = 0; i < count; ++i) {
-            const uint32_t sa = smem_base + stage * stage_bytes + i * kb_bytes;
-            const bool second = kb + i >= q.num_kb1;
-            const int k0 = (second ? kb + i - q.num_kb1 : kb + i) * K::kBlock;
-            const CUtensorMap* mA = &q.a[second ? 1 : 0];
-            const CUtensorMap* mB = &q.b[kTwoB ? static_cast<int>(rank) : (second ? 1 : 0)];
-            if (!q.a_mn) {
-              ptx::tma_load_3d_pair(sa, mA, fb, k0, m0, 0, pol);
+        const int x0 = for_a ? w.mt * 256 + static_cast<int>(rank) * 128
+                             : (kTwoB ? w.nt * (block_n >> 1) : w.nt * block_n + static_cast<int>(rank) * half_n);
+        const bool mn = (for_a ? q.a_mn : q.b_mn) != 0;
+        const int boxes = mn ? (for_a ? 128 : half_n) / static_cast<int>(K::kChunkElems) : 1;
+        const CUtensorMap* map1 = for_a ? &q.a[0] : &q.b[kTwoB ? static_cast<int>(rank) : 0];
+        const CUtensorMap* map2 = for_a ? &q.a[1] : &q.b[1];
+        const int kb1 = w.kb1, num_kb1 = q.num_kb1;
+        for (int kb = w.kb0; kb < kb1; kb += per_stage) {
+          if (!ready) {
+            ok = narrow_wait(empty_bar(stage), phase ^ 1u, abort_flag, p, kStatusProducerTimeout);
+            if (!ok) break;
+          }
+          const uint32_t fb = full0 + 8u * stage;
+          uint32_t dst = my_base + stage * stage_bytes;
+          const int count = min(per_stage, kb1 - kb);
+          if (for_a) ptx::mbar_expect_tx_cluster(fb, count * kb_bytes);
+          if (++stage == stages) { stage = 0; phase ^= 1u; }
+          ready = ptx::mbar_test_wait(empty_bar(stage), phase ^ 1u);
+          for (int i = kb; i < kb + count; ++i, dst += kb_bytes) {
+            const bool second = !kTwoB && i >= num_kb1;
+            const int k0 = (second ? i - num_kb1 : i) * K::kBlock;
+            const CUtensorMap* map = second ? map2 : map1;
+            if (!mn) {
+              ptx::tma_load_3d_pair(dst, map, fb, k0, x0, 0, pol);
+              if (my_groups == 2) ptx::tma_load_3d_pair(dst + half_bytes, map, fb, k0, x0 + n_step, 0, pol);
             } else {
-#pragma unroll
-              for (int c = 0; c < 128 / static_cast<int>(K::kChunkElems); ++c)
-                ptx::tma_load_3d_pair(sa + c * K::kChunkBytes, mA, fb, m0 + c * K::kChunkElems, k0, 0, pol);
-            }
-            for (int g = 0; g < groups; ++g) {
-              const uint32_t sb = sa + kNarrowABytes + g * half_bytes;
-              const int ng = n0 + g * n_step;
-              if (!q.b_mn) {
-                ptx::tma_load_3d_pair(sb, mB, fb, k0, ng, 0, pol);
-              } else {
-                for (int c = 0; c < half_n / static_cast<int>(K::kChunkElems); ++c)
-                  ptx::tma_load_3d_pair(sb + c * K::kChunkBytes, mB, fb, ng + c * K::kChunkElems, k0, 0, pol);
-              }
+              for (int g = 0; g < my_groups; ++g)
+                for (int c = 0; c < boxes; ++c)
+                  ptx::tma_load_3d_pair(dst + g * half_bytes + c * K::kChunkBytes, map, fb,
+                                        x0 + g * n_step + c * static_cast<int>(K::kChunkElems), k0, 0, pol);
             }
           }
-          if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
         }
       }
       // every release the leader's commits still owe this CTA must land before exit
@@ -502,6 +511,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
     if (lane == 0 && rank == 0 && my_group < groups) {
       const uint64_t stage_step = stage_bytes >> 4;
       const uint64_t kb_step = kb_bytes >> 4;
+      uint32_t ready = 0;
       int stage = 0;
       uint32_t phase = 0;
       int slot = my_group;
@@ -521,11 +531,18 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
         const uint32_t tmem_d = tmem_base + static_cast<uint32_t>(slot * kMaxBlockN);
         uint32_t accumulate = 0u;
         for (int kb = w.kb0; kb < w.kb1; kb += p.kb_per_stage) {
-          ok = narrow_wait(full_bar(stage), phase, abort_flag, p, kStatusMmaTimeout);
-          if (!ok) break;
+          // `ready`: the probe of this stage's barrier made a stage ago, its latency hidden behind the
+          // MMAs between
+          if (!ready) {
+            ok = narrow_wait(full_bar(stage), phase, abort_flag, p, kStatusMmaTimeout);
+            if (!ok) break;
+          }
           const int count = min(p.kb_per_stage, w.kb1 - kb);
           uint64_t da = a_desc0 + stage * stage_step;
           uint64_t db = b_desc0 + stage * stage_step;
+          const uint32_t freed = stage;
+          if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
+          ready = ptx::mbar_test_wait(full_bar(stage), phase);
           for (int i = 0; i < count; ++i, da += kb_step, db += kb_step) {
             ptx::mma_narrow_2cta<kKind>(tmem_d, da, db, idesc, accumulate);
             accumulate = 1u;
@@ -533,8 +550,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
             for (int ks = 1; ks < 4; ++ks)
               ptx::mma_narrow_2cta<kKind>(tmem_d, da + ks * a_step, db + ks * b_step, idesc, 1u);
           }
-          ptx::mma_commit_2cta_mask(empty_bar(stage), 3);   // the stage is free, in both CTAs
-          if (++stage == p.num_stages) { stage = 0; phase ^= 1u; }
+          ptx::mma_commit_2cta_mask(empty_bar(freed), 3);   // the stage is free, in both CTAs
         }
         if (!ok) break;
         ptx::mma_commit_2cta_mask(tfull_bar(slot), 3);      // the accumulator is complete, in both CTAs

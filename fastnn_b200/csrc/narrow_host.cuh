@@ -433,7 +433,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   p.total_units = static_cast<int>(units);
   // one thread issues a group's MMAs, and a stage's wait and commit cost it as much as an MMA or two: two
   // k-blocks a stage, except for wide tiles, whose two threads have twice the clocks for the same work
-  p.kb_per_stage = p.groups == 2 ? 1 : (tunables().kb_per_stage >= 1 && tunables().kb_per_stage <= 4 ? tunables().kb_per_stage : 2);
+  p.kb_per_stage = p.groups == 2 || l.epi == kEpiGatedGrad ? 1 : (tunables().kb_per_stage >= 1 && tunables().kb_per_stage <= 4 ? tunables().kb_per_stage : 2);
   const size_t stage = p.kb_per_stage * (kNarrowABytes + static_cast<size_t>(p.groups) * half_n * 128);
   const size_t fixed = narrow_fixed_bytes(l.epi);
   const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
@@ -749,12 +749,15 @@ int quantize_launch(const void* x, long long ld, int8_t* q, float* scale, int ro
   const int v = 16 / static_cast<int>(sizeof(T));
   const bool vec = rows_addressable(x, ld, sizeof(T)) && cols % v == 0 && (reinterpret_cast<uintptr_t>(q) & (v - 1)) == 0;
   const T* src = static_cast<const T*>(x);
-  // a warp holds 32 * kQuantHeld vectors of a row; longer rows take a block each
-  const bool warp = cols <= 32 * kQuantHeld * v;
+  // rows that a warp holds whole take a warp each, longer ones a block
+  const bool warp = cols <= 32 * (vec ? kQuantHeldLong : kQuantHeld) * v;
+  const bool shorter = cols <= 32 * kQuantHeld * v;
   const int per = kQuantThreads / 32;
   const int grid = warp ? (rows + per - 1) / per : rows;
-  auto* k = warp ? (vec ? quantize_rows_kernel<T, 32, true> : quantize_rows_kernel<T, 32, false>)
-                 : (vec ? quantize_rows_kernel<T, kQuantThreads, true> : quantize_rows_kernel<T, kQuantThreads, false>);
+  auto* k = quantize_rows_kernel<T, kQuantThreads, false, kQuantHeld>;
+  if (vec) k = !warp ? quantize_rows_kernel<T, kQuantThreads, true, kQuantHeld>
+                     : (shorter ? quantize_rows_kernel<T, 32, true, kQuantHeld> : quantize_rows_kernel<T, 32, true, kQuantHeldLong>);
+  else if (warp) k = quantize_rows_kernel<T, 32, false, kQuantHeld>;
   return launch_dependent(k, static_cast<unsigned>(grid), kQuantThreads, 0, s, src, ld, q, scale, rows, cols);
 }
 

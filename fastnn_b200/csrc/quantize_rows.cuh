@@ -6,8 +6,9 @@
 // zero: q = 0, scale = 0.  A row that holds a NaN or an infinity gets q = 0 and scale = NaN, so that a
 // product with it is NaN in that row and in no other.
 // The pass is bound by memory (the input is read once, a byte an element written): a row is held in
-// registers between the maximum and the rounding, up to kQuantHeld vectors a thread; what a longer row
-// has beyond that is read again, from L2.
+// registers between the maximum and the rounding, up to kHeld vectors a thread; what a longer row has
+// beyond that is read again, from L2.  A warp takes a row where that holds all of it (16 vectors a lane: 8 KiB
+// of row in flight for a warp and no block-wide barrier), a block the longer ones.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -18,7 +19,8 @@
 namespace fnn {
 
 constexpr int kQuantThreads = 256;
-constexpr int kQuantHeld = 4;
+constexpr int kQuantHeld = 4;         // vectors a thread holds of a short row, or of one a block shares
+constexpr int kQuantHeldLong = 16;    // of a row of up to 16 * 512 bytes that a warp takes alone
 
 template <typename T>
 __device__ __forceinline__ void quant_unpack(const uint4& w, float (&v)[16 / sizeof(T)]) {
@@ -41,7 +43,7 @@ __device__ __forceinline__ int quant_one(float x, float inv) { return __float2in
 
 // kPerRow threads share a row (32: a warp, kQuantThreads: the block).  kVec: rows and outputs in whole
 // 16-byte vectors of the input.
-template <typename T, int kPerRow, bool kVec>
+template <typename T, int kPerRow, bool kVec, int kHeld>
 __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* __restrict__ x, long long ld,
                                                                       int8_t* __restrict__ q,
                                                                       float* __restrict__ scale, int rows, int cols) {
@@ -57,21 +59,21 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* _
 
   // the magnitudes' bit patterns order as the magnitudes do, NaN above infinity
   uint32_t top = 0;
-  uint4 held[kQuantHeld];
+  uint4 held[kHeld];
   if constexpr (kVec) {
 #pragma unroll
-    for (int i = 0; i < kQuantHeld; ++i) {
+    for (int i = 0; i < kHeld; ++i) {
       const int v = part + i * kPerRow;
       held[i] = v < vecs ? __ldg(reinterpret_cast<const uint4*>(src) + v) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < kQuantHeld; ++i) {
+    for (int i = 0; i < kHeld; ++i) {
       float f[kVec ? 16 / sizeof(T) : 1];
       quant_unpack<T>(held[i], f);
 #pragma unroll
       for (int j = 0; j < kV; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
     }
-    for (int v = part + kQuantHeld * kPerRow; v < vecs; v += kPerRow) {
+    for (int v = part + kHeld * kPerRow; v < vecs; v += kPerRow) {
       float f[kVec ? 16 / sizeof(T) : 1];
       quant_unpack<T>(__ldg(reinterpret_cast<const uint4*>(src) + v), f);
 #pragma unroll
@@ -106,11 +108,11 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* _
       else reinterpret_cast<uint32_t*>(dst)[v] = b[0];
     };
 #pragma unroll
-    for (int i = 0; i < kQuantHeld; ++i) {
+    for (int i = 0; i < kHeld; ++i) {
       const int v = part + i * kPerRow;
       if (v < vecs) put(held[i], v);
     }
-    for (int v = part + kQuantHeld * kPerRow; v < vecs; v += kPerRow)
+    for (int v = part + kHeld * kPerRow; v < vecs; v += kPerRow)
       put(__ldg(reinterpret_cast<const uint4*>(src) + v), v);
   } else {
     for (int c = part; c < cols; c += kPerRow)
