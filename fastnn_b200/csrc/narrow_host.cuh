@@ -749,9 +749,10 @@ int quantize_launch(const void* x, long long ld, int8_t* q, float* scale, int ro
   const int v = 16 / static_cast<int>(sizeof(T));
   const bool vec = rows_addressable(x, ld, sizeof(T)) && cols % v == 0 && (reinterpret_cast<uintptr_t>(q) & (v - 1)) == 0;
   const T* src = static_cast<const T*>(x);
-  // rows that a warp holds whole take a warp each, longer ones a block
-  const bool warp = cols <= 32 * (vec ? kQuantHeldLong : kQuantHeld) * v;
+  // rows that a warp holds whole take a warp each, longer ones a block, and so do a few rows, whose loads a
+  // block has in flight all at once (1 row of 4096: 1.4 against 2.9 us)
   const bool shorter = cols <= 32 * kQuantHeld * v;
+  const bool warp = shorter || (vec && rows >= kQuantManyRows && cols <= 32 * kQuantHeldLong * v);
   const int per = kQuantThreads / 32;
   const int grid = warp ? (rows + per - 1) / per : rows;
   auto* k = quantize_rows_kernel<T, kQuantThreads, false, kQuantHeld>;

@@ -14,12 +14,15 @@
 #include <cuda_fp16.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 #include "ptx_sm100.cuh"
 
 namespace fnn {
 
 constexpr int kQuantThreads = 256;
 constexpr int kQuantHeld = 4;         // vectors a thread holds of a short row, or of one a block shares
+constexpr int kQuantManyRows = 1184;  // eight warps for each SM
 constexpr int kQuantHeldLong = 16;    // of a row of up to 16 * 512 bytes that a warp takes alone
 
 template <typename T>
@@ -39,7 +42,35 @@ __device__ __forceinline__ void quant_unpack(const uint4& w, float (&v)[16 / siz
   }
 }
 
-__device__ __forceinline__ int quant_one(float x, float inv) { return __float2int_rn(__fmul_rn(x, inv)); }
+// The integer nearest to the FP32 product x * inv, ties to even, in the low byte: |x * inv| <= 127.5, so
+// adding 1.5 * 2^23 leaves it in the last bits of the sum.  (The product is rounded first, as the
+// definition says: no fused multiply-add.)  A conversion instruction runs at a quarter of this rate.
+__device__ __forceinline__ uint32_t quant_one(float x, float inv) {
+  return __float_as_uint(__fadd_rn(__fmul_rn(x, inv), 12582912.0f));
+}
+__device__ __forceinline__ uint32_t quant_pack4(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+// The largest magnitude of a vector as a bit pattern; 16-bit types two at a time, in the upper and the
+// lower half of `top` (quant_top joins them).
+template <typename T>
+__device__ __forceinline__ uint32_t quant_max(uint32_t top, const uint4& w) {
+  const uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    if constexpr (sizeof(T) == 4) top = max(top, q[i] & 0x7fffffffu);
+    else top = __vmaxu2(top, q[i] & 0x7fff7fffu);
+  }
+  return top;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t quant_top(uint32_t top) {
+  if constexpr (sizeof(T) == 4) return top;
+  const uint32_t m = max(top >> 16, top & 0xffffu);
+  if constexpr (std::is_same<T, __half>::value)
+    return __float_as_uint(__half2float(__ushort_as_half(static_cast<unsigned short>(m)))) & 0x7fffffffu;
+  else return m << 16;
+}
 
 // kPerRow threads share a row (32: a warp, kQuantThreads: the block).  kVec: rows and outputs in whole
 // 16-byte vectors of the input.
@@ -67,18 +98,10 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* _
       held[i] = v < vecs ? __ldg(reinterpret_cast<const uint4*>(src) + v) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      float f[kVec ? 16 / sizeof(T) : 1];
-      quant_unpack<T>(held[i], f);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-    }
-    for (int v = part + kHeld * kPerRow; v < vecs; v += kPerRow) {
-      float f[kVec ? 16 / sizeof(T) : 1];
-      quant_unpack<T>(__ldg(reinterpret_cast<const uint4*>(src) + v), f);
-#pragma unroll
-      for (int j = 0; j < kV; ++j) top = max(top, __float_as_uint(f[j]) & 0x7fffffffu);
-    }
+    for (int i = 0; i < kHeld; ++i) top = quant_max<T>(top, held[i]);
+    for (int v = part + kHeld * kPerRow; v < vecs; v += kPerRow)
+      top = quant_max<T>(top, __ldg(reinterpret_cast<const uint4*>(src) + v));
+    top = quant_top<T>(top);
   } else {
     for (int c = part; c < cols; c += kPerRow)
       top = max(top, __float_as_uint(static_cast<float>(src[c])) & 0x7fffffffu);
@@ -101,9 +124,12 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* _
       float f[kVec ? 16 / sizeof(T) : 1];
       quant_unpack<T>(w, f);
       uint32_t b[2] = {0, 0};
+      if (live) {
 #pragma unroll
-      for (int j = 0; j < kV; ++j)
-        b[j >> 2] |= (static_cast<uint32_t>(live ? quant_one(f[j], inv) : 0) & 0xffu) << ((j & 3) * 8);
+        for (int j = 0; j < kV; j += 4)
+          b[j >> 2] = quant_pack4(quant_one(f[j], inv), quant_one(f[j + 1], inv), quant_one(f[j + 2], inv),
+                                  quant_one(f[j + 3], inv));
+      }
       if constexpr (kV == 8) reinterpret_cast<uint2*>(dst)[v] = make_uint2(b[0], b[1]);
       else reinterpret_cast<uint32_t*>(dst)[v] = b[0];
     };
@@ -116,7 +142,7 @@ __global__ void __launch_bounds__(kQuantThreads) quantize_rows_kernel(const T* _
       put(__ldg(reinterpret_cast<const uint4*>(src) + v), v);
   } else {
     for (int c = part; c < cols; c += kPerRow)
-      dst[c] = static_cast<int8_t>(live ? quant_one(static_cast<float>(src[c]), inv) : 0);
+      dst[c] = static_cast<int8_t>(live ? quant_one(static_cast<float>(src[c]), inv) & 0xffu : 0u);
   }
 }
 
