@@ -906,49 +906,53 @@ __global__ void __launch_bounds__(256) narrow_reduce_kernel(const __grid_constan
 
 // ------------------------------------------------------------------- row packing ---
 // Copies rows that TMA cannot address (a base or a row stride that is no multiple of 16 bytes) into a
-// buffer whose rows are.  Every destination word is put together from the two aligned source words it
-// straddles, so reads and writes are whole 32-bit words whatever the offset.
+// buffer whose rows are.  A thread puts 16 destination bytes together from the five aligned source words
+// they straddle, so reads are whole words and writes whole vectors whatever the offset.
 struct PackItem {
   const uint8_t* src;
   uint8_t* dst;
-  long long src_pitch, dst_pitch;    // bytes; dst_pitch a multiple of 16
+  long long src_pitch;               // bytes
   int rows, row_bytes, first_block;
+  FastDiv by_vecs;                   // 16-byte vectors of a destination row
 };
 constexpr int kMaxPack = 8;
 struct PackParams {
   PackItem it[kMaxPack];
   int count;
 };
-constexpr int kPackWords = 4 * 256;                  // destination words of one block (rows are not shared)
+constexpr int kPackVecs = 2;                         // vectors of one thread
 __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ PackParams p) {
   ptx::grid_dep_wait();
   ptx::grid_dep_launch_dependents();
   int i = 0;
   while (i + 1 < p.count && static_cast<int>(blockIdx.x) >= p.it[i + 1].first_block) ++i;
   const PackItem& q = p.it[i];
-  const int words = static_cast<int>(q.dst_pitch >> 2);
-  const long long total = static_cast<long long>(q.rows) * words;
-  const long long base = static_cast<long long>(blockIdx.x - q.first_block) * kPackWords + threadIdx.x;
-  const uintptr_t last = (reinterpret_cast<uintptr_t>(q.src) + (q.rows - 1) * q.src_pitch + q.row_bytes - 1) & ~uintptr_t(3);
+  const int vecs = static_cast<int>(q.by_vecs.d);
+  const int first = (static_cast<int>(blockIdx.x) - q.first_block) * 256 * kPackVecs + static_cast<int>(threadIdx.x);
+  // the last aligned word that holds a byte of the matrix; a word with none of its bytes is not read
+  const uintptr_t last = (reinterpret_cast<uintptr_t>(q.src) + static_cast<long long>(q.rows - 1) * q.src_pitch +
+                          q.row_bytes - 1) & ~uintptr_t(3);
 #pragma unroll
-  for (int k = 0; k < kPackWords / 256; ++k) {
-    const long long idx = base + k * 256;
-    if (idx >= total) break;
-    const long long r = idx / words;
-    const int w = static_cast<int>(idx - r * words);
-    uint32_t v = 0;
-    if (w * 4 < q.row_bytes) {
-      const uintptr_t s = reinterpret_cast<uintptr_t>(q.src) + r * q.src_pitch + w * 4;
-      const uintptr_t lo = s & ~uintptr_t(3);
-      // words that hold at least one byte of the matrix: the aligned word below an allocation's first
-      // byte, or the one that ends past its last, lies in the same 4-byte word as that byte
-      const uint32_t a = *reinterpret_cast<const uint32_t*>(lo);
-      const uint32_t b = (lo + 4 <= last) ? *reinterpret_cast<const uint32_t*>(lo + 4) : 0u;
-      v = __funnelshift_r(a, b, static_cast<uint32_t>(s & 3) * 8);
-      const int left = q.row_bytes - w * 4;
-      if (left < 4) v &= (1u << (left * 8)) - 1u;
+  for (int k = 0; k < kPackVecs; ++k) {
+    const int idx = first + k * 256;
+    const int r = div_by(idx, q.by_vecs);
+    if (r >= q.rows) break;
+    const int v = idx - r * vecs;
+    const uintptr_t s = reinterpret_cast<uintptr_t>(q.src) + r * q.src_pitch + v * 16;
+    const uintptr_t lo = s & ~uintptr_t(3);
+    uint32_t w[5];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = lo + 4 * j <= last ? *reinterpret_cast<const uint32_t*>(lo + 4 * j) : 0u;
+    const uint32_t shift = static_cast<uint32_t>(s & 3) * 8;
+    const int left = q.row_bytes - v * 16;           // bytes of the row from here on
+    uint32_t o[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      o[j] = __funnelshift_r(w[j], w[j + 1], shift);
+      const int mine = left - 4 * j;
+      if (mine < 4) o[j] = mine <= 0 ? 0u : o[j] & ((1u << (mine * 8)) - 1u);
     }
-    *reinterpret_cast<uint32_t*>(q.dst + r * q.dst_pitch + w * 4) = v;
+    *reinterpret_cast<uint4*>(q.dst + (static_cast<long long>(r) * vecs + v) * 16) = make_uint4(o[0], o[1], o[2], o[3]);
   }
 }
 

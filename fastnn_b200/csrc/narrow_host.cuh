@@ -110,7 +110,8 @@ struct Carver {
 
 struct Packer {
   fnn::PackParams p;
-  int blocks = 0;
+  long long blocks = 0;
+  bool too_large = false;
   Packer() { std::memset(&p, 0, sizeof(p)); }
   // m as TMA can address it: itself, or a copy in the workspace with rows padded to 16 bytes
   Mat fit(Carver& ws, const Mat& m, int bytes, bool pack) {
@@ -122,15 +123,18 @@ struct Packer {
       it.src = static_cast<const uint8_t*>(m.p);
       it.dst = static_cast<uint8_t*>(const_cast<void*>(out.p));
       it.src_pitch = m.ld * bytes;
-      it.dst_pitch = pitch;
       it.rows = m.rows;
       it.row_bytes = m.cols * bytes;
-      it.first_block = blocks;
-      blocks += static_cast<int>((m.rows * (pitch >> 2) + fnn::kPackWords - 1) / fnn::kPackWords);
+      it.by_vecs = fnn::fast_div(static_cast<int>(pitch >> 4));
+      it.first_block = static_cast<int>(blocks);
+      const long long vecs = m.rows * (pitch >> 4);
+      if (vecs > 0x7fffffffll - 256 * fnn::kPackVecs) too_large = true;      // 32 GiB of one operand
+      blocks += (vecs + 256 * fnn::kPackVecs - 1) / (256 * fnn::kPackVecs);
     }
     return out;
   }
   int launch(cudaStream_t s) {
+    if (too_large || blocks > 0x7fffffffll) return -1;
     if (blocks == 0) return 0;
     return launch_dependent(fnn::pack_rows_kernel, static_cast<unsigned>(blocks), 256, 0, s, p);
   }
