@@ -13,12 +13,18 @@
 // distributed shared memory, apply the epilogue and write -- no workspace, no second kernel, the same
 // bits every time.  A CTA asks for at most half of an SM, so that a CTA's start and end lie under its
 // neighbour's stream, and so that the next kernel's CTAs find room while this one's last are running.
+//
+// Between the two products of a block of at most 32 tokens the hidden rows are kept as a sum of two
+// 16-bit values, h = hi + lo: the second product takes both as tokens of their own and adds their results,
+// at no weight byte more, so that the only rounding of the block that counts is its output's.  (With many
+// tokens that would be twice the tensor work; there h is rounded once.)
 #pragma once
 #include "narrow_gemm_tcgen05.cuh"
 
 namespace fnn {
 
 constexpr int kSkinnyTokens = 128;                  // tokens of a tile, at most
+constexpr int kSkinnyFoldTokens = 32;               // tokens whose hidden rows are kept in two parts; twice that fits a tile
 // Producer, MMA issuer, and four to sixteen warps that drain the accumulator and apply the epilogue: at
 // 128 tokens and a short K the epilogue is most of a CTA's life, with a few tokens more warps only start
 // and meet later.
@@ -36,6 +42,8 @@ struct SkinnyParams {
   int t_tiles;               // token tiles
   int n_mma;                 // tokens of a tile, a multiple of 16
   int num_kb, split, num_stages, tmem_cols;
+  int fold;                  // > 0: the first product writes the low parts of its output this many rows on,
+                             // the second adds the rows this far on to its own
   int early_w;               // the weights may be read before the kernel ahead of this one has finished
   int act, is_bf16;
   const float* row_scale;
@@ -250,7 +258,7 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
     const int tid = static_cast<int>(threadIdx.x) - 64;
     const int r = tid % kQuads * 4;
     const int c = r0 + r;
-    const int tokens = c < p.n ? min(p.tokens - t0, p.n_mma) : 0;
+    const int tokens = c < p.n ? min((kEpi == kEpiStore && p.fold > 0 ? p.fold : p.tokens) - t0, p.n_mma) : 0;
     float cs[4], more[4];
     if constexpr (kEpi == kEpiScaled || kEpi == kEpiScaledGated) {
 #pragma unroll
@@ -267,6 +275,14 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
       float v[4], u[4];
       skinny_sum<kKind>(smem_gen + off, smem_base + off, p.split, v);
       if constexpr (kTwo) skinny_sum<kKind>(smem_gen + off + 256, smem_base + off + 256, p.split, u);
+      if constexpr (kEpi == kEpiStore) {
+        if (p.fold > 0) {                              // one token tile: the row is in this CTA's reach
+          const uint32_t low = off + static_cast<uint32_t>(p.fold) * 512u;
+          skinny_sum<kKind>(smem_gen + low, smem_base + low, p.split, u);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) v[j] += u[j];
+        }
+      }
       if constexpr (kEpi == kEpiGated) {
         if (p.out[1] != nullptr) {
           skinny_put<OutT>(p.out[1], p.out_ld[1], p.vec_out[1], t, c, p.n, v);
@@ -277,6 +293,14 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
 #pragma unroll
           for (int j = 0; j < 4; ++j) v[j] = gate_act<kAct>(v[j]) * u[j];
         });
+        if (p.fold > 0) {
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float hi = static_cast<float>(static_cast<OutT>(v[j]));
+            u[j] = isfinite(hi) ? v[j] - hi : 0.0f;    // nothing to add to an overflow or a NaN
+          }
+          skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t + p.fold, c, p.n, u);
+        }
       } else if constexpr (kEpi != kEpiStore) {
         const float rs = __ldg(p.row_scale + t);
         for_act(p.act, [&](auto tag) {

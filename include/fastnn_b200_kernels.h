@@ -338,7 +338,7 @@ FASTNN_B200_API int fastnn_b200_gemm_splitk_static(int layout, const float* a, c
  * FP32 product of this library).  act: none, ReLU, GELU(erf) or SiLU.  x may be a row-strided view (ld_x
  * elements, >= d_model); everything else is dense.  Both projections, the activation and the product
  * are one launch, the second product another; only act(gate) * up reaches memory between them, rounded
- * to the operands' type.  gate and up (both or neither NULL) receive x . Wg^T and x . Wu^T
+ * to the operands' type (for up to 32 tokens of 16 bits as a sum of two such values).  gate and up (both or neither NULL) receive x . Wg^T and x . Wu^T
  * [rows,d_ff], which the backward pass takes.  FastNN has no gated block; this stands beside
  * fastnn_b200_linear_forward (Linear + GELU, src/nn/linear.rs:55-88).
  * rows = 0 is a call without work.  Rows whose stride is no multiple of 16 bytes, and unaligned
