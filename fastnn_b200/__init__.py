@@ -5,7 +5,7 @@ package loads it and offers the thin host wrappers FastNN's ``cuda_backend`` mod
 (``cuda_matmul``, ``cuda_matmul_nt`` ...), operating on torch CUDA tensors.  There is no
 CPU fallback: importing works anywhere, computing needs the library and a B200.
 """
-from ._lib import LibraryMissing, lib, library_path  # noqa: F401
+from ._lib import LibraryMissing, binding, lib, library_path  # noqa: F401
 from .cuda_backend import (  # noqa: F401
     ACT_GELU, ACT_NONE, ACT_RELU, ACT_SILU, NN, NT, TN, CudaError, attention_forward, conv2d_backward, conv2d_forward, cuda_init, cuda_matmul, cuda_matmul_batched,
     cuda_matmul_batched_nt, cuda_matmul_batched_tn, cuda_matmul_nt, cuda_matmul_tn, device_status,

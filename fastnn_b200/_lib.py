@@ -94,3 +94,20 @@ def lib() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = handle
     return _lib
+
+
+_binding = None
+
+
+def binding():
+    """The torch binding (csrc/binding.cpp), linked against the library.  Raises LibraryMissing if absent."""
+    global _binding
+    if _binding is None:
+        lib()
+        try:
+            from . import _binding as module
+        except ImportError as exc:
+            raise LibraryMissing(f"{os.path.join(_HERE, '_binding.so')} cannot be loaded ({exc}): build it with "
+                                 "`python -m fastnn_b200.build`") from exc
+        _binding = module
+    return _binding

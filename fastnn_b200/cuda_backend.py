@@ -12,7 +12,7 @@ import ctypes
 
 import torch
 
-from ._lib import lib
+from ._lib import binding, lib
 
 NN, NT, TN = 0, 1, 2
 ACT_NONE, ACT_RELU, ACT_GELU = 0, 1, 2
@@ -331,67 +331,14 @@ def gru_pack_weights(w_ih, w_hh, b_ih=None, b_hh=None):
 
 
 # ---- gated feed-forward block and 8-bit products ---------------------------------------------
-# These run on torch's current stream unless ``stream`` (an integer, as elsewhere in this module) names
-# another; outputs and workspace then come from that stream's share of torch's allocator.  Their
-# workspace is an ordinary torch tensor: captured into a graph it lives in the graph's pool.
-
-_DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
-_GATE_ACTS = (ACT_NONE, ACT_RELU, ACT_GELU, ACT_SILU)
-
+# Checks, outputs, workspace and call are native (csrc/binding.cpp).  These run on torch's current stream
+# unless ``stream`` (an integer, as elsewhere in this module) names another; outputs and workspace then
+# come from that stream's share of torch's allocator.  Their workspace is an ordinary torch tensor:
+# captured into a graph it lives in the graph's pool.  Bad arguments are ValueErrors, a call that the
+# library refuses is a CudaError.
 
 def _as_current(stream):
     return torch.cuda.stream(torch.cuda.ExternalStream(int(stream)))
-
-
-def _row_stride(t, cols, name):
-    """Row stride of a tensor [.., cols] whose rows are contiguous and evenly spaced."""
-    if t.is_contiguous():
-        return cols
-    if t.stride(-1) == 1 or cols == 1:
-        if t.numel() <= cols:
-            return cols
-        try:
-            ld = int(t.view(-1, cols).stride(0))
-        except RuntimeError:
-            ld = 0
-        if ld >= cols:
-            return ld
-    raise ValueError(f"{name}: rows must be contiguous, evenly spaced and not overlap")
-
-
-def _check_like(t, name, dtype, device, shape):
-    if t.dtype is not dtype or t.get_device() != device or not t.is_contiguous():
-        raise ValueError(f"{name}: expected a contiguous {dtype} tensor on cuda:{device}")
-    if t.shape != shape:
-        raise ValueError(f"{name}: expected shape {tuple(shape)}, got {tuple(t.shape)}")
-
-
-def _on_current_device(t):
-    """The tensor's device index, with the library initialised there."""
-    dev = t.get_device()
-    if dev not in _initialised or torch.cuda.current_device() != dev:
-        _ensure_ctx(t)
-    return dev
-
-
-def _ffn_shapes(x, w_gate, w_up, w_down, act):
-    dtype = x.dtype
-    code = _DTYPE_CODE.get(dtype)
-    if code is None or not x.is_cuda or x.dim() < 1:
-        raise ValueError("x: expected a float32, float16 or bfloat16 CUDA tensor")
-    if act not in _GATE_ACTS:
-        raise ValueError("act must be ACT_NONE, ACT_RELU, ACT_GELU or ACT_SILU")
-    shape = w_gate.shape
-    if len(shape) != 2 or 0 in shape:
-        raise ValueError("w_gate must be [d_ff, d_model], neither of them 0")
-    f, d = shape
-    if x.shape[-1] != d:
-        raise ValueError(f"Expected input features {d}")
-    dev = _on_current_device(x)
-    _check_like(w_gate, "w_gate", dtype, dev, shape)
-    _check_like(w_up, "w_up", dtype, dev, shape)
-    _check_like(w_down, "w_down", dtype, dev, (d, f))
-    return code, d, f, dev
 
 
 def gated_ffn_forward(x, w_gate, w_up, w_down, act=ACT_SILU, return_pre=False, out=None, stream=None):
@@ -399,32 +346,11 @@ def gated_ffn_forward(x, w_gate, w_up, w_down, act=ACT_SILU, return_pre=False, o
     w_down [d_model, d_ff] as Linear stores weights (two halves of one fused matrix will do); all bfloat16,
     all float16, or all float32 (TF32 multiply).  Both projections, the activation and the product are one
     launch.  With ``return_pre`` returns (y, gate, up): the projections gated_ffn_backward takes.  ``out``
-    must not share memory with the inputs."""
+    must not share memory with the inputs.  x may be a strided view with contiguous, evenly spaced rows."""
     if stream is not None:
         with _as_current(stream):
-            return gated_ffn_forward(x, w_gate, w_up, w_down, act, return_pre, out)
-    code, d, f, dev = _ffn_shapes(x, w_gate, w_up, w_down, act)
-    ld = _row_stride(x, d, "x")
-    rows = x.numel() // d
-    px, pg, pu, pd = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
-    if out is None:
-        y = torch.empty_like(x, memory_format=torch.contiguous_format)
-    else:
-        _check_like(out, "out", x.dtype, dev, x.shape)
-        y = out
-    gate = up = None
-    if return_pre:
-        gate = x.new_empty(x.shape[:-1] + (f,))
-        up = torch.empty_like(gate)
-    handle = lib()
-    nbytes = handle.fastnn_b200_gated_ffn_workspace(
-        code, rows, d, f, 0, 1 if (px | pg | pu | pd | ld * x.element_size()) & 15 else 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    if handle.fastnn_b200_gated_ffn_forward(code, px, ld, pg, pu, pd, y.data_ptr(), gate.data_ptr() if return_pre else 0,
-                                            up.data_ptr() if return_pre else 0, rows, d, f, act, ws.data_ptr(), nbytes,
-                                            torch._C._cuda_getCurrentRawStream(dev)) != 0:
-        raise CudaError("CUDA gated_ffn_forward failed")
-    return (y, gate, up) if return_pre else y
+            return binding().gated_ffn_forward(x, w_gate, w_up, w_down, act, return_pre, out)
+    return binding().gated_ffn_forward(x, w_gate, w_up, w_down, act, return_pre, out)
 
 
 def gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act=ACT_SILU, stream=None):
@@ -432,30 +358,8 @@ def gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act=ACT_SILU, stre
     gate and up [.., d_ff].  Equal inputs give equal bits."""
     if stream is not None:
         with _as_current(stream):
-            return gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act)
-    code, d, f, dev = _ffn_shapes(x, w_gate, w_up, w_down, act)
-    dtype, shape = x.dtype, x.shape
-    ld_x = _row_stride(x, d, "x")
-    rows = x.numel() // d
-    if dy.dtype is not dtype or dy.get_device() != dev or dy.shape != shape:
-        raise ValueError("dy: expected a tensor like x")
-    ld_dy = _row_stride(dy, d, "dy")
-    saved = shape[:-1] + (f,)
-    _check_like(gate, "gate", dtype, dev, saved)
-    _check_like(up, "up", dtype, dev, saved)
-    p_dy, px, p_gate, p_up = dy.data_ptr(), x.data_ptr(), gate.data_ptr(), up.data_ptr()
-    pg, pu, pd = w_gate.data_ptr(), w_up.data_ptr(), w_down.data_ptr()
-    bits = (ld_x | ld_dy) * x.element_size() | p_dy | px | p_gate | p_up | pg | pu | pd
-    dx = torch.empty_like(x, memory_format=torch.contiguous_format)
-    dwg, dwu, dwd = torch.empty_like(w_gate), torch.empty_like(w_up), torch.empty_like(w_down)
-    handle = lib()
-    nbytes = handle.fastnn_b200_gated_ffn_workspace(code, rows, d, f, 1, 1 if bits & 15 else 0)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=x.device)
-    if handle.fastnn_b200_gated_ffn_backward(code, p_dy, ld_dy, px, ld_x, p_gate, p_up, pg, pu, pd, dx.data_ptr(),
-                                             dwg.data_ptr(), dwu.data_ptr(), dwd.data_ptr(), rows, d, f, act,
-                                             ws.data_ptr(), nbytes, torch._C._cuda_getCurrentRawStream(dev)) != 0:
-        raise CudaError("CUDA gated_ffn_backward failed")
-    return dx, dwg, dwu, dwd
+            return binding().gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act)
+    return binding().gated_ffn_backward(dy, x, gate, up, w_gate, w_up, w_down, act)
 
 
 def quantize_rows(x, stream=None):
@@ -465,80 +369,18 @@ def quantize_rows(x, stream=None):
     scales are per token, for a weight [out, in] per output channel."""
     if stream is not None:
         with _as_current(stream):
-            return quantize_rows(x)
-    code = _DTYPE_CODE.get(x.dtype)
-    shape = x.shape
-    if code is None or not x.is_cuda or len(shape) < 1 or shape[-1] < 1:
-        raise ValueError("x: expected a float32, float16 or bfloat16 CUDA tensor with at least one column")
-    dev = _on_current_device(x)
-    cols = shape[-1]
-    ld = _row_stride(x, cols, "x")
-    q = torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format)
-    scale = x.new_empty(shape[:-1], dtype=torch.float32)
-    if lib().fastnn_b200_quantize_rows(code, x.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), x.numel() // cols, cols,
-                                       torch._C._cuda_getCurrentRawStream(dev)) != 0:
-        raise CudaError("CUDA quantize_rows failed")
-    return q, scale
-
-
-def _int8_shapes(xq, x_scale, wq, act, out_dtype):
-    shape = xq.shape
-    if xq.dtype is not torch.int8 or not xq.is_cuda or len(shape) < 1 or not xq.is_contiguous():
-        raise ValueError("xq: expected a contiguous int8 CUDA tensor")
-    if act not in _GATE_ACTS:
-        raise ValueError("act must be ACT_NONE, ACT_RELU, ACT_GELU or ACT_SILU")
-    code = _DTYPE_CODE.get(out_dtype)
-    if code is None:
-        raise ValueError("out_dtype must be float32, float16 or bfloat16")
-    w_shape = wq.shape
-    if len(w_shape) != 2 or 0 in w_shape:
-        raise ValueError("weights must be [out_features, in_features], neither of them 0")
-    n, k = w_shape
-    if shape[-1] != k:
-        raise ValueError(f"Expected input features {k}")
-    if k > 131071:
-        raise ValueError("in_features above 131071 could overflow the 32-bit sums")
-    dev = _on_current_device(xq)
-    _check_like(x_scale, "x_scale", torch.float32, dev, shape[:-1])
-    return code, xq.numel() // k, k, n, dev, shape[:-1] + (n,)
-
-
-def _check_int8_weight(name, w, scale, dev, n, k):
-    _check_like(w, name, torch.int8, dev, (n, k))
-    _check_like(scale, name + " scale", torch.float32, dev, (n,))
-
-
-def _int8_workspace(rows, k, n, gated, bits, device):
-    """(tensor to keep, pointer, bytes); rows of a multiple of 16 bytes on such bases need none."""
-    if not (bits | k) & 15:
-        return None, 0, 0
-    nbytes = lib().fastnn_b200_int8_workspace(rows, k, n, gated, 1)
-    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
-    return ws, ws.data_ptr(), nbytes
+            return binding().quantize_rows(x)
+    return binding().quantize_rows(x)
 
 
 def int8_linear_forward(xq, x_scale, wq, w_scale, bias=None, act=ACT_NONE, out_dtype=torch.float32, out=None,
                         stream=None):
     """y = act(x_scale[t] * w_scale[o] * (xq . wq^T) + bias) for xq [.., in] and wq [out, in] as quantize_rows
-    makes them; bias [out] float32.  The integer sums are exact; y [.., out] has ``out_dtype``."""
+    makes them; bias [out] float32.  The integer sums are exact (in <= 131071); y [.., out] has ``out_dtype``."""
     if stream is not None:
         with _as_current(stream):
-            return int8_linear_forward(xq, x_scale, wq, w_scale, bias, act, out_dtype, out)
-    code, rows, k, n, dev, shape = _int8_shapes(xq, x_scale, wq, act, out_dtype)
-    _check_int8_weight("wq", wq, w_scale, dev, n, k)
-    if bias is not None:
-        _check_like(bias, "bias", torch.float32, dev, (n,))
-    px, pw = xq.data_ptr(), wq.data_ptr()
-    if out is None:
-        out = xq.new_empty(shape, dtype=out_dtype)
-    else:
-        _check_like(out, "out", out_dtype, dev, shape)
-    ws, pws, nbytes = _int8_workspace(rows, k, n, 0, px | pw, xq.device)
-    if lib().fastnn_b200_int8_linear_forward(px, x_scale.data_ptr(), pw, w_scale.data_ptr(),
-                                             0 if bias is None else bias.data_ptr(), out.data_ptr(), code, rows, k, n,
-                                             act, pws, nbytes, torch._C._cuda_getCurrentRawStream(dev)) != 0:
-        raise CudaError("CUDA int8_linear_forward failed")
-    return out
+            return binding().int8_linear_forward(xq, x_scale, wq, w_scale, bias, act, out_dtype, out)
+    return binding().int8_linear_forward(xq, x_scale, wq, w_scale, bias, act, out_dtype, out)
 
 
 def int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act=ACT_SILU, out_dtype=torch.float32,
@@ -547,21 +389,8 @@ def int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act=AC
     half of a gated block in 8-bit integers, in one launch; xq [.., in], weights [out, in], h [.., out]."""
     if stream is not None:
         with _as_current(stream):
-            return int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act, out_dtype, out)
-    code, rows, k, n, dev, shape = _int8_shapes(xq, x_scale, wq_gate, act, out_dtype)
-    _check_int8_weight("wq_gate", wq_gate, gate_scale, dev, n, k)
-    _check_int8_weight("wq_up", wq_up, up_scale, dev, n, k)
-    px, pg, pu = xq.data_ptr(), wq_gate.data_ptr(), wq_up.data_ptr()
-    if out is None:
-        out = xq.new_empty(shape, dtype=out_dtype)
-    else:
-        _check_like(out, "out", out_dtype, dev, shape)
-    ws, pws, nbytes = _int8_workspace(rows, k, n, 1, px | pg | pu, xq.device)
-    if lib().fastnn_b200_int8_gated_forward(px, x_scale.data_ptr(), pg, gate_scale.data_ptr(), pu, up_scale.data_ptr(),
-                                            out.data_ptr(), code, rows, k, n, act, pws, nbytes,
-                                            torch._C._cuda_getCurrentRawStream(dev)) != 0:
-        raise CudaError("CUDA int8_gated_forward failed")
-    return out
+            return binding().int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act, out_dtype, out)
+    return binding().int8_gated_forward(xq, x_scale, wq_gate, gate_scale, wq_up, up_scale, act, out_dtype, out)
 
 
 def gemm_ex(layout, a_ptr, b_ptr, c_ptr, m, n, k, batch, lda, ldb, ldc, sa, sb, sc,
