@@ -315,24 +315,26 @@ NarrowKernel<N> pair_kernel(int kind, int epi, int out_code) {
 }
 
 typedef void (*SkinnyKernel)(fnn::SkinnyParams);
-SkinnyKernel skinny_kernel(int kind, int epi, int out_code) {
+// w_mn: the weights are stored [k, rows] (the gradients' products).
+SkinnyKernel skinny_kernel(int kind, int epi, int out_code, bool w_mn) {
   using namespace fnn;
+  const bool bf = out_code == FASTNN_B200_BF16;
   if (kind == kKindF16) {
-    const bool bf = out_code == FASTNN_B200_BF16;
-    if (epi == kEpiStore) return bf ? &narrow_skinny_kernel<kKindF16, kEpiStore, __nv_bfloat16> : &narrow_skinny_kernel<kKindF16, kEpiStore, __half>;
-    if (epi == kEpiGated) return bf ? &narrow_skinny_kernel<kKindF16, kEpiGated, __nv_bfloat16> : &narrow_skinny_kernel<kKindF16, kEpiGated, __half>;
+    if (epi == kEpiStore && !w_mn) return bf ? &narrow_skinny_kernel<kKindF16, kEpiStore, __nv_bfloat16, false> : &narrow_skinny_kernel<kKindF16, kEpiStore, __half, false>;
+    if (epi == kEpiStore) return bf ? &narrow_skinny_kernel<kKindF16, kEpiStore, __nv_bfloat16, true> : &narrow_skinny_kernel<kKindF16, kEpiStore, __half, true>;
+    if (epi == kEpiGated && !w_mn) return bf ? &narrow_skinny_kernel<kKindF16, kEpiGated, __nv_bfloat16, false> : &narrow_skinny_kernel<kKindF16, kEpiGated, __half, false>;
+    if (epi == kEpiGatedGrad && w_mn) return bf ? &narrow_skinny_kernel<kKindF16, kEpiGatedGrad, __nv_bfloat16, true> : &narrow_skinny_kernel<kKindF16, kEpiGatedGrad, __half, true>;
   } else if (kind == kKindTf32) {
-    if (epi == kEpiStore) return &narrow_skinny_kernel<kKindTf32, kEpiStore, float>;
-    if (epi == kEpiGated) return &narrow_skinny_kernel<kKindTf32, kEpiGated, float>;
-  } else {
+    if (epi == kEpiStore) return w_mn ? &narrow_skinny_kernel<kKindTf32, kEpiStore, float, true> : &narrow_skinny_kernel<kKindTf32, kEpiStore, float, false>;
+    if (epi == kEpiGated && !w_mn) return &narrow_skinny_kernel<kKindTf32, kEpiGated, float, false>;
+    if (epi == kEpiGatedGrad && w_mn) return &narrow_skinny_kernel<kKindTf32, kEpiGatedGrad, float, true>;
+  } else if (!w_mn) {
     if (epi == kEpiScaled)
-      return out_code == FASTNN_B200_F32 ? &narrow_skinny_kernel<kKindI8, kEpiScaled, float>
-             : (out_code == FASTNN_B200_BF16 ? &narrow_skinny_kernel<kKindI8, kEpiScaled, __nv_bfloat16>
-                                             : &narrow_skinny_kernel<kKindI8, kEpiScaled, __half>);
+      return out_code == FASTNN_B200_F32 ? &narrow_skinny_kernel<kKindI8, kEpiScaled, float, false>
+             : (bf ? &narrow_skinny_kernel<kKindI8, kEpiScaled, __nv_bfloat16, false> : &narrow_skinny_kernel<kKindI8, kEpiScaled, __half, false>);
     if (epi == kEpiScaledGated)
-      return out_code == FASTNN_B200_F32 ? &narrow_skinny_kernel<kKindI8, kEpiScaledGated, float>
-             : (out_code == FASTNN_B200_BF16 ? &narrow_skinny_kernel<kKindI8, kEpiScaledGated, __nv_bfloat16>
-                                             : &narrow_skinny_kernel<kKindI8, kEpiScaledGated, __half>);
+      return out_code == FASTNN_B200_F32 ? &narrow_skinny_kernel<kKindI8, kEpiScaledGated, float, false>
+             : (bf ? &narrow_skinny_kernel<kKindI8, kEpiScaledGated, __nv_bfloat16, false> : &narrow_skinny_kernel<kKindI8, kEpiScaledGated, __half, false>);
   }
   return nullptr;
 }
@@ -347,9 +349,9 @@ int narrow_init() {
           FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
         if (auto k = pair_kernel<fnn::kNarrowMaxProblems>(kind, epi, c))
           FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
-        SkinnyKernel sk = skinny_kernel(kind, epi, c);
-        if (sk != nullptr)
-          FNN_CUDA_OK(cudaFuncSetAttribute(sk, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSkinnySmem)));
+        for (bool mn : {false, true})
+          if (SkinnyKernel k = skinny_kernel(kind, epi, c, mn))
+            FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSkinnySmem)));
       }
   return 0;
 }
@@ -487,8 +489,18 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
 // machine once: CTA pairs then have fewer tiles than SMs and cannot cut K under a gated epilogue (200
 // tokens, 1024 x 1024 block: 12 against 18 us; 2048 x 2048: 20 / 26; 4096 x 16384, 512 tiles: 120 / 97).
 // set_policy(3) and (4) force it and CTA pairs.
-bool use_skinny(int tokens, int n, int epi) {
+// The gradients' products can share a launch on CTA pairs, whose K splits have no limit and whose epilogue
+// reads the saved projections ahead.  There (`grad`) this form is for tokens whose parts are kept in two,
+// and for weights that are worth streaming on their own, over enough CTAs (200 tokens, 1024 x 1024: 21.9
+// against 24.9 us; 59 tokens, 4085 x 14336: 281 / 306; 127 tokens,
+// 3336 x 768: 27 / 44; but 140 tokens, 320 x 2496: 38 / 29).
+bool use_skinny(int tokens, int n, int k, int epi, bool grad) {
   if (t_policy.policy == 3 || t_policy.policy == 4) return t_policy.policy == 3;
+  if (grad && tokens > fnn::kSkinnyFoldTokens) {
+    const long long ctas = 1ll * ceil_div(n, 128) * ceil_div(tokens, fnn::kSkinnyTokens) * (tokens > 64 ? 4 : 8);
+    const bool long_k = epi == fnn::kEpiGatedGrad && k >= 1024;      // the pairs' gated epilogue cannot split it
+    if (!long_k && (1ll * n * k < (1 << 20) || ctas < 64)) return false;
+  }
   if (tokens <= fnn::kSkinnyTokens) return true;
   return tokens <= 512 && 1ll * ceil_div(n, epi_gated(epi) ? 64 : 128) * ceil_div(tokens, fnn::kSkinnyTokens) <= 256;
 }
@@ -524,14 +536,21 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
   p.t_tiles = ceil_div(t.m, kSkinnyTokens);
   p.n_mma = ceil_div(ceil_div(t.m, p.t_tiles), 16) * 16;
   p.t_tiles = ceil_div(t.m, p.n_mma);
-  p.num_kb = ceil_div(t.k, kblock);
+  p.num_kb1 = ceil_div(t.k, kblock);
+  p.num_kb = p.num_kb1 + (t.k2 > 0 ? ceil_div(t.k2, kblock) : 0);
   const int tiles = ceil_div(t.n, tile_rows);
   p.split = skinny_split(1ll * tiles * p.t_tiles, p.num_kb, p.n_mma);
-  bool ok = encode_narrow(&p.x, l.in, t.a[0].p, t.a[0].cols, t.a[0].rows, 1, t.a[0].ld * l.in.bytes,
-                          t.a[0].ld * l.in.bytes * t.a[0].rows, kblock, p.n_mma, kSwz128);
-  for (int j = 0; j < (two ? 2 : 1); ++j)
-    ok = ok && encode_narrow(&p.w[j], l.in, t.b[j].p, t.b[j].cols, t.b[j].rows, 1, t.b[j].ld * l.in.bytes,
-                             t.b[j].ld * l.in.bytes * t.b[j].rows, kblock, tile_rows, kSwz128);
+  bool ok = true;
+  auto operand = [&](CUtensorMap* map, const Mat& m, uint32_t box1, MapSwizzle swz) {
+    const uint64_t pitch = m.ld * l.in.bytes;
+    return m.rows == 0 || encode_narrow(map, l.in, m.p, m.cols, m.rows, 1, pitch, pitch * m.rows, kblock, box1, swz);
+  };
+  for (int j = 0; j < 2; ++j) {
+    ok = ok && operand(&p.x[j], t.a[j], p.n_mma, kSwz128);
+    // t.b as launch_pair takes it: [rows, k], or [k, rows] when b_mn
+    ok = ok && operand(&p.w[j], t.b[j], t.b_mn ? kblock : tile_rows,
+                       t.b_mn && l.in.kind == kKindTf32 ? kSwz128Atom32 : kSwz128);
+  }
   if (!ok) return -1;
   DType out;
   if (!dtype_of(l.out_code, &out)) return -1;
@@ -540,6 +559,9 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
     p.out_ld[j] = t.out_ld[j];
     p.vec_out[j] = (reinterpret_cast<uintptr_t>(t.out[j]) % (4 * out.bytes) == 0 && t.out_ld[j] % 4 == 0) ? 1 : 0;
   }
+  p.aux[0] = t.aux[0]; p.aux[1] = t.aux[1]; p.aux_ld = t.aux_ld;
+  p.vec_aux = (reinterpret_cast<uintptr_t>(t.aux[0]) | reinterpret_cast<uintptr_t>(t.aux[1])) % (4 * out.bytes) == 0 &&
+              t.aux_ld % 4 == 0 ? 1 : 0;
   const int slice_kb = ceil_div(p.num_kb, p.split);
   const size_t stage = kNarrowABytes + static_cast<size_t>(p.n_mma) * 128;
   int stages = static_cast<int>((kSkinnySmem - skinny_smem_bytes(p.n_mma, 0)) / stage);
@@ -563,7 +585,7 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
   const size_t floor_bytes = sm_smem / (512 / p.tmem_cols + 1) + 1;
   size_t smem = skinny_smem_bytes(p.n_mma, stages);
   if (smem < floor_bytes) smem = floor_bytes;
-  SkinnyKernel k = skinny_kernel(l.in.kind, l.epi, l.out_code);
+  SkinnyKernel k = skinny_kernel(l.in.kind, l.epi, l.out_code, t.b_mn);
   if (k == nullptr || smem > kSkinnySmem) return -1;
   const long long grid = 1ll * tiles * p.t_tiles * p.split;
   if (grid > 0x7fffffffll) return -1;
@@ -612,8 +634,8 @@ int ffn_forward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, cu
   const Mat wg = pk.fit(ws, a.wg, e, must_pack(a.wg));
   const Mat wu = pk.fit(ws, a.wu, e, must_pack(a.wu));
   const Mat wd = pk.fit(ws, a.wd, e, must_pack(a.wd));
-  const bool skinny1 = use_skinny(a.rows, a.f, fnn::kEpiGated);
-  const bool skinny2 = use_skinny(a.rows, a.d, fnn::kEpiStore);
+  const bool skinny1 = use_skinny(a.rows, a.f, a.d, fnn::kEpiGated, false);
+  const bool skinny2 = use_skinny(a.rows, a.d, a.f, fnn::kEpiStore, false);
   // Hidden rows in two parts for up to 32 tokens, where it costs no more than the second product's tokens
   // (24 tokens, 1024 x 4096: 11.9 -> 12.5 us; 64 tokens: 13.5 -> 16.8).
   const int fold = skinny1 && skinny2 && e == 2 && a.rows <= fnn::kSkinnyFoldTokens ? a.rows : 0;
@@ -661,17 +683,27 @@ int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, c
   const Mat wg = pk.fit(ws, a.wg, e, must_pack(a.wg));
   const Mat wu = pk.fit(ws, a.wu, e, must_pack(a.wu));
   const Mat wd = pk.fit(ws, a.wd, e, must_pack(a.wd));
-  const bool pack_aux = must_pack(a.gate) || must_pack(a.up);     // one stride for both
+  const bool skinny1 = use_skinny(a.rows, a.f, a.d, fnn::kEpiGatedGrad, true);
+  const bool skinny2 = use_skinny(a.rows, a.d, a.f, fnn::kEpiStore, true);
+  // dgate, dup and h in two parts each, as the forward pass keeps its hidden rows
+  const int fold = skinny1 && skinny2 && e == 2 && a.rows <= fnn::kSkinnyFoldTokens ? a.rows : 0;
+  const int h_rows = a.rows + fold;
+  // CTA pairs read the saved projections by TMA, with one stride for both
+  const bool pack_aux = !skinny1 && (must_pack(a.gate) || must_pack(a.up));
   const Mat gate = pk.fit(ws, a.gate, e, pack_aux);
   const Mat up = pk.fit(ws, a.up, e, pack_aux);
   const long long h_ld = round_up(1ll * a.f * e, 16) / e;
-  const size_t h_bytes = static_cast<size_t>(h_ld) * a.rows * e;
+  const size_t h_bytes = static_cast<size_t>(h_ld) * h_rows * e;
   void* dg = ws.take(h_bytes);
   void* du = ws.take(h_bytes);
   void* h = ws.take(h_bytes);
   const int kblock = 128 / e;
   const Mat none{nullptr, 0, 0, 0};
-  const Mat mdg{dg, h_ld, a.rows, a.f}, mdu{du, h_ld, a.rows, a.f}, mh{h, h_ld, a.rows, a.f};
+  // rows of the high parts, or all rows; and the low parts' rows, none without them
+  auto part = [&](void* p, int first, int rows) {
+    if (rows == 0) return none;
+    return Mat{p == nullptr ? nullptr : static_cast<uint8_t*>(p) + static_cast<size_t>(h_ld) * first * e, h_ld, rows, a.f};
+  };
 
   NarrowTask t1;                                   // dh = dy . Wd, never stored
   t1.a[0] = dy; t1.a[1] = none; t1.b[0] = wd; t1.b[1] = none;
@@ -681,32 +713,40 @@ int ffn_backward(DeviceState* st, const FfnArgs& a, Carver& ws, bool pack_all, c
   for (long long& ld : t1.out_ld) ld = h_ld;
   t1.aux[0] = gate.p; t1.aux[1] = up.p; t1.aux_ld = gate.ld;
 
+  // dx, then dWg, dWu, dWd; with low parts a second range of K adds their products
   NarrowTask g[4];
-  g[0].a[0] = mdg; g[0].a[1] = mdu; g[0].b[0] = wg; g[0].b[1] = wu;       // dx
+  g[0].a[0] = part(dg, 0, h_rows); g[0].a[1] = part(du, 0, h_rows); g[0].b[0] = wg; g[0].b[1] = wu;
   g[0].b_mn = true;
-  g[0].m = a.rows; g[0].n = a.d; g[0].k = a.f; g[0].k2 = a.f;
+  g[0].m = h_rows; g[0].n = a.d; g[0].k = a.f; g[0].k2 = a.f;
   g[0].out[0] = a.dx; g[0].out_ld[0] = a.d;
-  for (int i = 1; i <= 2; ++i) {                                          // dWg, dWu
-    g[i].a[0] = i == 1 ? mdg : mdu; g[i].a[1] = none; g[i].b[0] = x; g[i].b[1] = none;
+  for (int i = 1; i <= 2; ++i) {
+    void* d = i == 1 ? dg : du;
+    g[i].a[0] = part(d, 0, a.rows); g[i].a[1] = part(d, a.rows, fold);
+    g[i].b[0] = x; g[i].b[1] = fold > 0 ? x : none;
     g[i].a_mn = g[i].b_mn = true;
-    g[i].m = a.f; g[i].n = a.d; g[i].k = a.rows;
+    g[i].m = a.f; g[i].n = a.d; g[i].k = a.rows; g[i].k2 = fold;
     g[i].out[0] = i == 1 ? a.dwg : a.dwu; g[i].out_ld[0] = a.d;
   }
-  g[3].a[0] = dy; g[3].a[1] = none; g[3].b[0] = mh; g[3].b[1] = none;     // dWd
+  g[3].a[0] = dy; g[3].a[1] = fold > 0 ? dy : none; g[3].b[0] = part(h, 0, a.rows); g[3].b[1] = part(h, a.rows, fold);
   g[3].a_mn = g[3].b_mn = true;
-  g[3].m = a.d; g[3].n = a.f; g[3].k = a.rows;
+  g[3].m = a.d; g[3].n = a.f; g[3].k = a.rows; g[3].k2 = fold;
   g[3].out[0] = a.dwd; g[3].out_ld[0] = a.f;
+  NarrowTask* group = skinny2 ? g + 1 : g;             // the products of the last launch
+  const int count = skinny2 ? 3 : 4;
   const int cl = clusters_of(st);
-  const NarrowPlan p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGatedGrad, false);
-  const NarrowPlan p2 = plan_narrow(g, 4, kblock, cl, fnn::kEpiStore, true);
-  reserve_partials(ws, g, 4, p2);
+  NarrowPlan p1{0};
+  if (!skinny1) p1 = plan_narrow(&t1, 1, kblock, cl, fnn::kEpiGatedGrad, false);
+  const NarrowPlan p2 = plan_narrow(group, count, kblock, cl, fnn::kEpiStore, true);
+  reserve_partials(ws, group, count, p2);
   if (dry) return 0;
   if (!ws.fits()) return -1;
   if (pk.launch(s) != 0) return -1;
   NarrowLaunch l{a.t, a.t.code, fnn::kEpiGatedGrad, a.act};
-  if (launch_pair<1>(st, l, &t1, 1, p1, s) != 0) return -1;
+  if ((skinny1 ? launch_skinny(st, l, t1, false, fold, s) : launch_pair<1>(st, l, &t1, 1, p1, s)) != 0) return -1;
   l.epi = fnn::kEpiStore;
-  return launch_pair<fnn::kNarrowMaxProblems>(st, l, g, 4, p2, s);
+  // Wg and Wu may be read early, as Wd in the forward pass
+  if (skinny2 && launch_skinny(st, l, g[0], true, fold, s) != 0) return -1;
+  return launch_pair<fnn::kNarrowMaxProblems>(st, l, group, count, p2, s);
 }
 
 bool ffn_sizes_ok(int rows, int d, int f) { return rows >= 0 && d >= 1 && f >= 1; }
@@ -746,7 +786,7 @@ int int8_product(DeviceState* st, const Int8Args& a, Carver& ws, bool pack_all, 
   if (pk.launch(s) != 0) return -1;
   NarrowLaunch l{kInt8, a.out_code, a.gated ? fnn::kEpiScaledGated : fnn::kEpiScaled, a.act};
   l.row_scale = a.xs; l.col_scale = a.ws; l.col_scale2 = a.ws2; l.bias = a.bias;
-  if (use_skinny(a.rows, a.n, l.epi)) return launch_skinny(st, l, t, false, 0, s);
+  if (use_skinny(a.rows, a.n, a.k, l.epi, false)) return launch_skinny(st, l, t, false, 0, s);
   const NarrowPlan p = plan_narrow(&t, 1, 128, clusters_of(st), l.epi, false);
   return launch_pair<1>(st, l, &t, 1, p, s);
 }

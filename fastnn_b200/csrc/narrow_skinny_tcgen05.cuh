@@ -1,6 +1,6 @@
 // The same products for few tokens (decoding): the weight's rows on the tensor core's M side.
 //
-//   out[t, r] = epilogue( sum_k x[t, k] * W[r, k] )
+//   out[t, r] = epilogue( sum_k x[t, k] * W[r, k] )         W stored [r, k], or [k, r] (the gradients')
 //
 // With up to 128 tokens the time is that of reading the weights once, so the form is chosen for bytes in
 // flight and for even shares of them; a few hundred are cut into equal tiles of at most 128, whose CTAs
@@ -34,16 +34,19 @@ constexpr int kSkinnyMaxStages = 8;
 constexpr int kSkinnyBarBytes = 256;
 
 struct SkinnyParams {
-  CUtensorMap w[2], x;
+  CUtensorMap w[2], x[2];    // [1]: the up weight of a gated product, or a second K range of both operands
   void* out[3];              // as NarrowProblem: the product, and for a gated one optionally gate and up
   long long out_ld[3];
   int vec_out[3];            // rows may be written four columns at a time
+  const void* aux[2];        // kEpiGatedGrad: the saved gate and up projections
+  long long aux_ld;
+  int vec_aux;
   int tokens, n;             // n: columns of one output
   int t_tiles;               // token tiles
   int n_mma;                 // tokens of a tile, a multiple of 16
-  int num_kb, split, num_stages, tmem_cols;
-  int fold;                  // > 0: the first product writes the low parts of its output this many rows on,
-                             // the second adds the rows this far on to its own
+  int num_kb, num_kb1, split, num_stages, tmem_cols;    // num_kb1: k-blocks of the first range
+  int fold;                  // > 0: a gated epilogue writes the low parts of its outputs this many rows on, a
+                             // plain one adds the rows this far on to its own
   int early_w;               // the weights may be read before the kernel ahead of this one has finished
   int act, is_bf16;
   const float* row_scale;
@@ -115,7 +118,36 @@ __device__ __forceinline__ void skinny_put(void* out, long long ld, int vec, int
   }
 }
 
-template <int kKind, int kEpi, typename OutT>
+// Four values of a saved projection's row.
+template <typename T>
+__device__ __forceinline__ void skinny_get(const void* src, long long ld, int vec, int t, int c, int n, float (&v)[4]) {
+  const T* at = static_cast<const T*>(src) + static_cast<long long>(t) * ld + c;
+  if (vec && c + 4 <= n) {
+    if constexpr (sizeof(T) == 4) {
+      const float4 f = __ldg(reinterpret_cast<const float4*>(at));
+      v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+    } else {
+      const uint2 w = __ldg(reinterpret_cast<const uint2*>(at));
+      const float2 a = unpack2<T>(w.x), b = unpack2<T>(w.y);
+      v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = c + j < n ? static_cast<float>(at[j]) : 0.0f;
+  }
+}
+
+// v as a 16-bit value, in v's place the rest: nothing to add to an overflow or a NaN.
+template <typename T>
+__device__ __forceinline__ void skinny_rest(float (&v)[4]) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float hi = static_cast<float>(static_cast<T>(v[j]));
+    v[j] = isfinite(hi) ? v[j] - hi : 0.0f;
+  }
+}
+
+template <int kKind, int kEpi, typename OutT, bool kWMn>
 __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(const __grid_constant__ SkinnyParams p) {
   using K = NarrowKind<kKind>;
   constexpr bool kTwo = kEpi == kEpiGated || kEpi == kEpiScaledGated;
@@ -152,11 +184,22 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
       ptx::tma_load_3d_hint(sa, &p.w[0], fb, kb * K::kBlock, r0, 0, pol);
       ptx::tma_load_3d_hint(sa + 64 * 128, &p.w[1], fb, kb * K::kBlock, r0, 0, pol);
     } else {
-      ptx::tma_load_3d_hint(sa, &p.w[0], fb, kb * K::kBlock, r0, 0, pol);
+      const bool second = kb >= p.num_kb1;
+      const CUtensorMap* map = &p.w[second ? 1 : 0];
+      const int k0 = (second ? kb - p.num_kb1 : kb) * K::kBlock;
+      if constexpr (kWMn) {
+#pragma unroll
+        for (int c = 0; c < 128 / static_cast<int>(K::kChunkElems); ++c)
+          ptx::tma_load_3d_hint(sa + c * K::kChunkBytes, map, fb, r0 + c * static_cast<int>(K::kChunkElems), k0, 0, pol);
+      } else {
+        ptx::tma_load_3d_hint(sa, map, fb, k0, r0, 0, pol);
+      }
     }
   };
   auto load_x = [&](int kb, int s) {
-    ptx::tma_load_3d(smem_base + s * stage_bytes + kNarrowABytes, &p.x, full_bar(s), kb * K::kBlock, t0, 0);
+    const bool second = !kTwo && kb >= p.num_kb1;
+    ptx::tma_load_3d(smem_base + s * stage_bytes + kNarrowABytes, &p.x[second ? 1 : 0], full_bar(s),
+                     (second ? kb - p.num_kb1 : kb) * K::kBlock, t0, 0);
   };
 
   int pre = 0;
@@ -203,8 +246,9 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      const uint32_t idesc = ptx::idesc_narrow<kKind>(128, p.n_mma, 0, 0, p.is_bf16);
-      const uint64_t a_desc0 = narrow_desc<kKind>(smem_base, 0);
+      const uint32_t idesc = ptx::idesc_narrow<kKind>(128, p.n_mma, kWMn ? 1 : 0, 0, p.is_bf16);
+      const uint64_t a_desc0 = narrow_desc<kKind>(smem_base, kWMn ? 1 : 0);
+      constexpr uint64_t kAStep = (kWMn ? K::kMnStep : 32u) >> 4;
       const uint64_t b_desc0 = narrow_desc<kKind>(smem_base + kNarrowABytes, 0);
       const uint64_t stage_step = stage_bytes >> 4;
       int stage = 0;
@@ -218,7 +262,7 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
         const uint64_t db = b_desc0 + stage * stage_step;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
-          ptx::mma_narrow_1cta<kKind>(tmem_base, da + ks * 2, db + ks * 2, idesc, accumulate);
+          ptx::mma_narrow_1cta<kKind>(tmem_base, da + ks * kAStep, db + ks * 2, idesc, accumulate);
           accumulate = 1u;
         }
         ptx::mma_commit_1cta(empty_bar(stage));
@@ -269,7 +313,19 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
         else more[j] = in && p.bias != nullptr ? __ldg(p.bias + c + j) : 0.0f;
       }
     }
-    for (int tl = slice * at_once + tid / kQuads; tl < tokens; tl += p.split * at_once) {
+    // the saved projections of a token come from memory while the one before it is computed
+    float g[4], gu[4];
+    auto load_aux = [&](int tl) {
+      if constexpr (kEpi == kEpiGatedGrad) {
+        if (tl < tokens) {
+          skinny_get<OutT>(p.aux[0], p.aux_ld, p.vec_aux, t0 + tl, c, p.n, g);
+          skinny_get<OutT>(p.aux[1], p.aux_ld, p.vec_aux, t0 + tl, c, p.n, gu);
+        }
+      }
+    };
+    const int step = p.split * at_once;
+    load_aux(slice * at_once + tid / kQuads);
+    for (int tl = slice * at_once + tid / kQuads; tl < tokens; tl += step) {
       const int t = t0 + tl;
       const uint32_t off = static_cast<uint32_t>(tl * 128 + r) * 4u;
       float v[4], u[4];
@@ -295,11 +351,34 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
         });
         if (p.fold > 0) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float hi = static_cast<float>(static_cast<OutT>(v[j]));
-            u[j] = isfinite(hi) ? v[j] - hi : 0.0f;    // nothing to add to an overflow or a NaN
-          }
+          for (int j = 0; j < 4; ++j) u[j] = v[j];
+          skinny_rest<OutT>(u);
           skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t + p.fold, c, p.n, u);
+        }
+      } else if constexpr (kEpi == kEpiGatedGrad) {
+        // v is dh: dgate = dh * up * act'(gate), dup = dh * act(gate), h = act(gate) * up
+        float o[3][4], here[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) { here[j] = g[j]; u[j] = gu[j]; }
+        load_aux(tl + step);
+        for_act(p.act, [&](auto tag) {
+          constexpr int kAct = decltype(tag)::value;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            float a, da;
+            gate_act_grad<kAct>(here[j], a, da);
+            o[0][j] = v[j] * u[j] * da;
+            o[1][j] = v[j] * a;
+            o[2][j] = a * u[j];
+          }
+        });
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+          skinny_put<OutT>(p.out[i], p.out_ld[i], p.vec_out[i], t, c, p.n, o[i]);
+          if (p.fold > 0) {
+            skinny_rest<OutT>(o[i]);
+            skinny_put<OutT>(p.out[i], p.out_ld[i], p.vec_out[i], t + p.fold, c, p.n, o[i]);
+          }
         }
       } else if constexpr (kEpi != kEpiStore) {
         const float rs = __ldg(p.row_scale + t);
@@ -314,7 +393,7 @@ __global__ void __launch_bounds__(kSkinnyMaxThreads, 2) narrow_skinny_kernel(con
           }
         });
       }
-      skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
+      if constexpr (kEpi != kEpiGatedGrad) skinny_put<OutT>(p.out[0], p.out_ld[0], p.vec_out[0], t, c, p.n, v);
     }
   }
   __syncwarp();
