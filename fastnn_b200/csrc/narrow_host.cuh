@@ -493,13 +493,13 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
 // reads the saved projections ahead.  There (`grad`) this form is for tokens whose parts are kept in two,
 // and for weights that are worth streaming on their own, over enough CTAs (200 tokens, 1024 x 1024: 21.9
 // against 24.9 us; 59 tokens, 4085 x 14336: 281 / 306; 127 tokens,
-// 3336 x 768: 27 / 44; but 140 tokens, 320 x 2496: 38 / 29).
+// 3336 x 768: 27 / 44; but 140 tokens, 320 x 2496: 38 / 29, and 500 tokens, 512 x 2048: 30 / 25).
 bool use_skinny(int tokens, int n, int k, int epi, bool grad) {
   if (t_policy.policy == 3 || t_policy.policy == 4) return t_policy.policy == 3;
   if (grad && tokens > fnn::kSkinnyFoldTokens) {
     const long long ctas = 1ll * ceil_div(n, 128) * ceil_div(tokens, fnn::kSkinnyTokens) * (tokens > 64 ? 4 : 8);
     const bool long_k = epi == fnn::kEpiGatedGrad && k >= 1024;      // the pairs' gated epilogue cannot split it
-    if (!long_k && (1ll * n * k < (1 << 20) || ctas < 64)) return false;
+    if (!long_k && (tokens > 320 || 1ll * n * k < (1 << 20) || ctas < 64)) return false;
   }
   if (tokens <= fnn::kSkinnyTokens) return true;
   return tokens <= 512 && 1ll * ceil_div(n, epi_gated(epi) ? 64 : 128) * ceil_div(tokens, fnn::kSkinnyTokens) <= 256;

