@@ -4,6 +4,7 @@
 
 namespace {
 
+constexpr size_t kSkinnyMinSmem = 73 * 1024;
 constexpr size_t kSkinnySmem = 115712;     // half of an SM's 228 KiB, less the 1 KiB reserved per CTA
 constexpr int kDefaultClusters = 74;       // CTA pairs of a B200, for size queries without a device
 
@@ -443,6 +444,7 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   const size_t stage = p.kb_per_stage * (kNarrowABytes + static_cast<size_t>(p.groups) * half_n * 128);
   const size_t fixed = narrow_fixed_bytes(l.epi);
   const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
+  if (stages < 1) return -1;
   p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;
   p.group_m = group_m;
   p.act = l.act;
@@ -454,7 +456,9 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   const int clusters = p.total_units < st->max_clusters ? p.total_units : st->max_clusters;
   const NarrowKernel<N> k = pair_kernel<N>(l.in.kind, l.epi, l.out_code);
   if (k == nullptr || clusters < 1) return -1;
-  if (launch_dependent(k, 2 * clusters, l.epi == kEpiGatedGrad ? kNarrowThreads<kEpiGatedGrad> : kNarrowThreads<kEpiStore>, fixed + p.num_stages * stage, stream, p) != 0) return -1;
+  // All of the SM's shared memory, whatever the stages need: the kernel takes all of tensor memory, and no
+  // CTA that wants columns too may come to wait for them beside it.
+  if (launch_dependent(k, 2 * clusters, l.epi == kEpiGatedGrad ? kNarrowThreads<kEpiGatedGrad> : kNarrowThreads<kEpiStore>, kMaxDynSmem, stream, p) != 0) return -1;
   t_last = LastCall{12, plan.block_n, t[0].split, 2 * clusters};
 
   NarrowReduceParams r;
@@ -579,12 +583,12 @@ int launch_skinny(DeviceState* st, const NarrowLaunch& l, const NarrowTask& t, b
   p.row_scale = l.row_scale; p.col_scale = l.col_scale; p.col_scale2 = l.col_scale2; p.bias = l.bias;
   p.status = st->status;
   p.spin_budget = st->spin_budget;
-  // Tensor memory is 512 columns: no more CTAs may share an SM than have their columns (a CTA that waits
-  // for columns while its cluster waits for it would never get them), which the shared memory enforces.
-  const size_t sm_smem = 228 * 1024;
-  const size_t floor_bytes = sm_smem / (512 / p.tmem_cols + 1) + 1;
+  // Tensor memory is 512 columns.  A CTA that waits for columns while its cluster waits for it, beside
+  // another such, would never get them, so CTAs that fit an SM together must never want more than 512
+  // together: at 73 KiB three of these share an SM, and beside the CTAs of the cluster split-K GEMM, which
+  // ask for 228 KiB / (512 / columns + 1) each, no mix that fits wants more.
   size_t smem = skinny_smem_bytes(p.n_mma, stages);
-  if (smem < floor_bytes) smem = floor_bytes;
+  if (smem < kSkinnyMinSmem) smem = kSkinnyMinSmem;
   SkinnyKernel k = skinny_kernel(l.in.kind, l.epi, l.out_code, t.b_mn);
   if (k == nullptr || smem > kSkinnySmem) return -1;
   const long long grid = 1ll * tiles * p.t_tiles * p.split;
