@@ -188,8 +188,11 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
   const int max_bn = epi == fnn::kEpiGatedGrad ? 256 : 512;
   for (int bn = min_bn; bn <= max_bn; bn *= 2) {
     if (want_bn >= min_bn && want_bn <= max_bn && bn != want_bn) continue;
-    const double per_kb = bn == 512 ? 1100.0 : (bn == 256 ? 620.0 : (bn == 128 ? 400.0 : 330.0));
-    const double drain = (epi == fnn::kEpiGatedGrad ? 6000.0 : 2500.0) * bn / 256.0;
+    const double per_kb = bn == 512 ? 1130.0 : (bn == 256 ? 620.0 : (bn == 128 ? 465.0 : 410.0));
+    // a tile's fixed part, and for 256 accumulator columns: a plain store is memory traffic, the others
+    // mostly arithmetic
+    static const double kDrain[5] = {1000.0, 2200.0, 13500.0, 6500.0, 3500.0};        // by kEpi*
+    const double drain = 1500.0 + kDrain[epi] * bn / 256.0;
     for (int parts = 1; parts <= (may_split ? 64 : 1); parts += parts < 8 ? 1 : (parts < 16 ? 2 : 8)) {
       const int len = ceil_div(max_kb, parts);                  // k-blocks of a unit, at most
       if (parts > 1 && len < 4) break;
@@ -224,8 +227,8 @@ PlanChoice choose_narrow(const NarrowTask* t, int count, int kblock, int cluster
           }
           if (sum > most) most = sum;
         }
-        // partial sums are written and read once, at a third of the cost while they stay in L2
-        const double reduce = partial > 0.0 ? 5000.0 + 2.0 * partial / (partial < 48e6 ? 10200.0 : 3400.0) : 0.0;
+        // partial sums are written and read once, at about half the cost while they stay in L2
+        const double reduce = partial > 0.0 ? 5000.0 + 2.0 * partial / (partial < 48e6 ? 6000.0 : 3400.0) : 0.0;
         const double cost = most + drain + reduce;
         if (cost < best) { best = cost; best_bn = bn; best_len = len; best_keep = keep != 0; }
       }

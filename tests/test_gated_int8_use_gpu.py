@@ -382,3 +382,54 @@ def test_train_then_quantise_and_serve(gpu):
         # and near the block it came from: 127 steps to the largest value of a row, on both operands
         ref = _block64(x[:t], *[m.bfloat16() for m in master])
         assert _rel(y, ref) <= 0.05
+
+
+def test_two_threads_on_two_streams(gpu):
+    """Calls from two host threads, each on its own stream and with its own kernel-form override (which
+    belongs to the calling thread), at the same time."""
+    import threading
+    import torch
+    cases = [_inputs(300, 512, 1024, torch.bfloat16, seed=1), _inputs(20, 1000, 520, torch.float16, seed=2)]
+
+    def work(x, wg, wu, wd):
+        y, gate, up = gpu.gated_ffn_forward(x, wg, wu, wd, return_pre=True)
+        q, s = gpu.quantize_rows(x)
+        wq, ws = gpu.quantize_rows(wg)
+        return (y,) + gpu.gated_ffn_backward(y, x, gate, up, wg, wu, wd) + (gpu.int8_linear_forward(q, s, wq, ws),)
+    want = [work(*c) for c in cases]
+    torch.cuda.synchronize()
+    bad, errors = [], []
+
+    def run(i):
+        try:
+            torch.cuda.set_device(0)
+            stream = torch.cuda.Stream()
+            with torch.cuda.stream(stream):
+                for _ in range(30):
+                    got = work(*cases[i])
+                    stream.synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i])):
+                        bad.append(i)
+        except Exception as exc:                             # reported by the thread that asserts
+            errors.append(exc)
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not errors and not bad
+
+
+def test_a_weight_used_twice_and_views_of_one_buffer(gpu):
+    import torch
+    for rows in (4, 300):
+        x, w, _, wd = _inputs(rows, 128, 256, torch.bfloat16)
+        want = _block64(x, w, w, wd)
+        assert _rel(gpu.gated_ffn_forward(x, w, w, wd), want) <= _tol(x)
+        square = _inputs(128, 128, 128, torch.bfloat16, seed=4)[0]
+        y, gate, up = gpu.gated_ffn_forward(square, square, square, square, return_pre=True)
+        assert _rel(y, _block64(square, square, square, square)) <= _tol(x)
+        dx, a, b, c = gpu.gated_ffn_backward(square, square, gate, up, square, square, square, act=gpu.ACT_SILU)
+        again = gpu.gated_ffn_backward(square.clone(), square.clone(), gate, up, square.clone(), square.clone(),
+                                       square.clone(), act=gpu.ACT_SILU)
+        assert all(torch.equal(p, q) for p, q in zip((dx, a, b, c), again))
