@@ -913,8 +913,9 @@ __global__ void __launch_bounds__(256) narrow_reduce_kernel(const __grid_constan
 
 // ------------------------------------------------------------------- row packing ---
 // Copies rows that TMA cannot address (a base or a row stride that is no multiple of 16 bytes) into a
-// buffer whose rows are.  A thread puts 16 destination bytes together from the five aligned source words
-// they straddle, so reads are whole words and writes whole vectors whatever the offset.
+// buffer whose rows are.  A thread puts 16 destination bytes together from the two aligned 16-byte blocks
+// they straddle, so reads and writes are whole vectors whatever the offset.  A block is read only if it
+// holds a byte of the matrix; what else it holds lies in the same 256-byte granule of device memory.
 struct PackItem {
   const uint8_t* src;
   uint8_t* dst;
@@ -936,9 +937,8 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ 
   const PackItem& q = p.it[i];
   const int vecs = static_cast<int>(q.by_vecs.d);
   const int first = (static_cast<int>(blockIdx.x) - q.first_block) * 256 * kPackVecs + static_cast<int>(threadIdx.x);
-  // the last aligned word that holds a byte of the matrix; a word with none of its bytes is not read
-  const uintptr_t last = (reinterpret_cast<uintptr_t>(q.src) + static_cast<long long>(q.rows - 1) * q.src_pitch +
-                          q.row_bytes - 1) & ~uintptr_t(3);
+  const uintptr_t last = reinterpret_cast<uintptr_t>(q.src) + static_cast<long long>(q.rows - 1) * q.src_pitch +
+                         q.row_bytes - 1;            // the matrix's last byte
 #pragma unroll
   for (int k = 0; k < kPackVecs; ++k) {
     const int idx = first + k * 256;
@@ -946,11 +946,19 @@ __global__ void __launch_bounds__(256) pack_rows_kernel(const __grid_constant__ 
     if (r >= q.rows) break;
     const int v = idx - r * vecs;
     const uintptr_t s = reinterpret_cast<uintptr_t>(q.src) + r * q.src_pitch + v * 16;
-    const uintptr_t lo = s & ~uintptr_t(3);
+    const uintptr_t lo = s & ~uintptr_t(15);
+    const uint32_t off = static_cast<uint32_t>(s & 15);
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (lo <= last) a = __ldg(reinterpret_cast<const uint4*>(lo));
+    if (off != 0 && lo + 16 <= last) b = __ldg(reinterpret_cast<const uint4*>(lo + 16));
+    // the words from the first that holds a wanted byte on
+    const bool two = (off & 8) != 0, one = (off & 4) != 0;
+    const uint32_t t[6] = {two ? a.z : a.x, two ? a.w : a.y, two ? b.x : a.z, two ? b.y : a.w, two ? b.z : b.x,
+                           two ? b.w : b.y};
     uint32_t w[5];
 #pragma unroll
-    for (int j = 0; j < 5; ++j) w[j] = lo + 4 * j <= last ? *reinterpret_cast<const uint32_t*>(lo + 4 * j) : 0u;
-    const uint32_t shift = static_cast<uint32_t>(s & 3) * 8;
+    for (int j = 0; j < 5; ++j) w[j] = one ? t[j + 1] : t[j];
+    const uint32_t shift = (off & 3) * 8;
     const int left = q.row_bytes - v * 16;           // bytes of the row from here on
     uint32_t o[4];
 #pragma unroll
