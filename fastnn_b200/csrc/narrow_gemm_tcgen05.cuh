@@ -39,17 +39,19 @@ enum : int {
   kEpiGated = 1,      // out0 = act(gate) * up, optionally out1 = gate, out2 = up
   kEpiGatedGrad = 2,  // acc = dh: out0 = dh * up * act'(gate), out1 = dh * act(gate), out2 = act(gate) * up
   kEpiScaled = 3,     // C = act(acc * row_scale * col_scale + bias)
-  kEpiScaledGated = 4 // C = act(gate * row_scale * col_scale) * (up * row_scale * col_scale2)
+  kEpiScaledGated = 4,// C = act(gate * row_scale * col_scale) * (up * row_scale * col_scale2)
+  kEpiGatedGradDeep = 5  // CTA pairs: kEpiGatedGrad with less staging and deeper stages
 };
+constexpr bool epi_grad(int epi) { return epi == kEpiGatedGrad || epi == kEpiGatedGradDeep; }
 // Activations of this file's epilogues (the public codes, kActSilu beyond the GEMM epilogue's own).
 constexpr int kActSilu = 5;
 
 // Epilogue warps, four for each TMEM lane quadrant: what an epilogue waits for (tensor memory, staging
 // tiles, fixed latencies) is covered by other warps, and with two for each quadrant a tile's drain took
 // 1.5 to 2 times as long (7.2 against 4 k clocks for 256 columns of 8-bit products).  The gradient
-// epilogue is bound by its memory traffic and has two with two sets of tiles each.
+// epilogue is bound by its memory traffic and has two with more tiles each.
 template <int kEpi>
-constexpr int kEpiWarps = kEpi == kEpiGatedGrad ? 8 : 16;
+constexpr int kEpiWarps = kEpi == kEpiGatedGrad || kEpi == kEpiGatedGradDeep ? 8 : 16;
 template <int kEpi>
 constexpr int kNarrowThreads = 32 * (kEpiWarps<kEpi> + 4);    // + two producers and two MMA issuers
 constexpr int kNarrowMaxProblems = 4;
@@ -58,12 +60,23 @@ constexpr int kNarrowABytes = 128 * 128;             // 128 rows x 128 bytes of 
 constexpr int kNarrowBarBytes = 512;
 constexpr int kNarrowGroupM = 8;                     // tile rows of a rasterisation group: 2048 rows
 // A staging tile is 32 rows of 64 bytes (in the 64-byte swizzle): 32 columns of 16 bits, 16 of 32.  An
-// epilogue warp owns one; a gradient epilogue's owns two sets of (gate, up, h).
+// epilogue warp owns one; a gradient epilogue's owns two sets of (gate, up, h),
+// or two tiles where K is deep.
 constexpr int kTile = 32 * 64;
 template <typename T>
 constexpr int kTileCols = 64 / static_cast<int>(sizeof(T));
+// Staging of one epilogue warp. kEpiGatedGrad has two sets of (gate, up, h) tiles, so that a chunk's loads
+// run under the chunk before it. kEpiGatedGradDeep has two tiles, and h goes through the first one once that
+// is stored: a chunk's loads and stores then wait for one another, which a long main loop covers, and the
+// room holds three stages of two k-blocks instead of four of one (256 columns).
+// Whole backward in bf16, two sets / deep, in turn on one GPU: 8192 tokens, d 4096, f 16384 5663 / 5515 us;
+// 2048 tokens of it 1401 / 1372; 8192 tokens, d 2048, f 8192 1429 / 1403; d 1536 (24 k-blocks), f 6144 907 / 907.
+// Below that the two sets win (both forms in one kernel with a branch): d 1280, f 5120 644 / 648; d 1024,
+// f 8192 831 / 849; d 256, f 1024 51.5 / 58.4.  They are kernels of their own because that branch cost 18
+// registers, and the 8192-token d 256 case 53.9 in place of 52.1 us.
 template <int kEpi>
-constexpr int kStagingWarp = kEpi == kEpiGatedGrad ? 6 * kTile : kTile;
+constexpr int kStagingWarp = kEpi == kEpiGatedGrad ? 6 * kTile : (kEpi == kEpiGatedGradDeep ? 2 * kTile : kTile);
+constexpr int kGradDeepMinKb = 24;
 
 // n / d for 0 <= n < 2^31 without a division (Granlund and Montgomery): every epilogue warp decodes every
 // tile, and four integer divisions were a third of a short-K tile's instructions.
@@ -383,7 +396,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kNarrowThreads<kEpi>
 narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
   using K = NarrowKind<kKind>;
   constexpr bool kTwoB = kEpi == kEpiGated || kEpi == kEpiScaledGated;
-  constexpr bool kGrad = kEpi == kEpiGatedGrad;
+  constexpr bool kDeep = kEpi == kEpiGatedGradDeep;      // see kStagingWarp
+  constexpr bool kGrad = kEpi == kEpiGatedGrad || kDeep;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (ptx::smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - ptx::smem_u32(smem_raw));
@@ -730,9 +744,9 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
                 more = live(wn, cn);
               }
               if (lane == 0) {
-                ptx::tma_store_wait_read<0>();               // every store so far has read its tiles
+                if (!kDeep || !fetched) ptx::tma_store_wait_read<0>();     // every store so far has read its tiles
                 if (!fetched) fetch_aux(w, c, set);
-                if (more) fetch_aux(wn, cn, set ^ 1);
+                if (!kDeep && more) fetch_aux(wn, cn, set ^ 1);
               }
               __syncwarp();
               ok = narrow_wait(aux_bar(ew, set), (set_phase >> set) & 1u, abort_flag, p, kStatusEpilogueTimeout);
@@ -740,6 +754,7 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
               if (!ok) break;
               set_phase ^= 1u << set;
               ptx::tmem_ld_wait();
+              [[maybe_unused]] uint32_t kept[16];            // kDeep: this lane's row of h, as stored
               for_act(p.act, [&](auto tag) {
                 constexpr int kAct = decltype(tag)::value;
 #pragma unroll
@@ -758,7 +773,15 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
                   }
                   tile_put8<OutT>(tiles, lane, j, gv);
                   tile_put8<OutT>(tiles + kTile, lane, j, uv);
-                  tile_put8<OutT>(tiles + 2 * kTile, lane, j, hv);
+                  if constexpr (!kDeep) {
+                    tile_put8<OutT>(tiles + 2 * kTile, lane, j, hv);
+                  } else if constexpr (sizeof(OutT) == 4) {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) kept[8 * j + i] = __float_as_uint(hv[i]);
+                  } else {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) kept[4 * j + i] = pack2<OutT>(hv[2 * i], hv[2 * i + 1]);
+                  }
                 }
               });
               ptx::fence_proxy_async_smem();
@@ -767,11 +790,28 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
                 const uint32_t ta = set_addr(set);
                 ptx::tma_store_3d(&q.out[0], ta, col0, m0, 0);
                 ptx::tma_store_3d(&q.out[1], ta + kTile, col0, m0, 0);
-                ptx::tma_store_3d(&q.out[2], ta + 2 * kTile, col0, m0, 0);
+                if constexpr (!kDeep) ptx::tma_store_3d(&q.out[2], ta + 2 * kTile, col0, m0, 0);
                 ptx::tma_store_commit();
+                if constexpr (kDeep) ptx::tma_store_wait_read<0>();
+              }
+              if constexpr (kDeep) {                         // h follows through the first tile
+                __syncwarp();
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                  *reinterpret_cast<uint4*>(tiles + tile_unit(lane, j)) =
+                      make_uint4(kept[4 * j], kept[4 * j + 1], kept[4 * j + 2], kept[4 * j + 3]);
+                ptx::fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                  ptx::tma_store_3d(&q.out[2], set_addr(0), col0, m0, 0);
+                  ptx::tma_store_commit();
+                  ptx::tma_store_wait_read<0>();
+                  if (more) fetch_aux(wn, cn, 0);
+                }
+              } else {
+                set ^= 1;
               }
               fetched = more;
-              set ^= 1;
             }
           } else {
             // 8-bit products: the scale of this lane's row, and the scales (and bias) of the columns,
@@ -850,8 +890,9 @@ narrow_pair_kernel(const __grid_constant__ NarrowParams<kProblems> p) {
 
 // Shared memory beside the stages.
 inline size_t narrow_fixed_bytes(int epi) {
-  const int staging = epi == kEpiGatedGrad ? kEpiWarps<kEpiGatedGrad> * kStagingWarp<kEpiGatedGrad>
-                                           : kEpiWarps<kEpiStore> * kStagingWarp<kEpiStore>;
+  const int staging = epi == kEpiGatedGrad       ? kEpiWarps<kEpiGatedGrad> * kStagingWarp<kEpiGatedGrad>
+                      : epi == kEpiGatedGradDeep ? kEpiWarps<kEpiGatedGradDeep> * kStagingWarp<kEpiGatedGradDeep>
+                                                 : kEpiWarps<kEpiStore> * kStagingWarp<kEpiStore>;
   return 1024 + static_cast<size_t>(staging) + kNarrowBarBytes;
 }
 

@@ -299,12 +299,14 @@ NarrowKernel<N> pair_kernel(int kind, int epi, int out_code) {
     if (epi == kEpiStore) return bf ? &narrow_pair_kernel<kKindF16, kEpiStore, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiStore, __half, N>;
     if constexpr (N == 1) {
       if (epi == kEpiGated) return bf ? &narrow_pair_kernel<kKindF16, kEpiGated, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiGated, __half, N>;
+      if (epi == kEpiGatedGradDeep) return bf ? &narrow_pair_kernel<kKindF16, kEpiGatedGradDeep, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiGatedGradDeep, __half, N>;
       if (epi == kEpiGatedGrad) return bf ? &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __nv_bfloat16, N> : &narrow_pair_kernel<kKindF16, kEpiGatedGrad, __half, N>;
     }
   } else if (kind == kKindTf32) {
     if (epi == kEpiStore) return &narrow_pair_kernel<kKindTf32, kEpiStore, float, N>;
     if constexpr (N == 1) {
       if (epi == kEpiGated) return &narrow_pair_kernel<kKindTf32, kEpiGated, float, N>;
+      if (epi == kEpiGatedGradDeep) return &narrow_pair_kernel<kKindTf32, kEpiGatedGradDeep, float, N>;
       if (epi == kEpiGatedGrad) return &narrow_pair_kernel<kKindTf32, kEpiGatedGrad, float, N>;
     }
   } else if constexpr (N == 1) {
@@ -347,7 +349,7 @@ SkinnyKernel skinny_kernel(int kind, int epi, int out_code, bool w_mn) {
 int narrow_init() {
   const int codes[3] = {FASTNN_B200_F32, FASTNN_B200_F16, FASTNN_B200_BF16};
   for (int kind = 0; kind <= 2; ++kind)
-    for (int epi = 0; epi <= 4; ++epi)
+    for (int epi = 0; epi <= 5; ++epi)
       for (int c : codes) {
         if (auto k = pair_kernel<1>(kind, epi, c))
           FNN_CUDA_OK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kMaxDynSmem)));
@@ -442,10 +444,13 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   p.count = count;
   p.total_units = static_cast<int>(units);
   // one thread issues a group's MMAs, and a stage's wait and commit cost it as much as an MMA or two: two
-  // k-blocks a stage, except for wide tiles, whose two threads have twice the clocks for the same work
-  p.kb_per_stage = p.groups == 2 || l.epi == kEpiGatedGrad ? 1 : (tunables().kb_per_stage >= 1 && tunables().kb_per_stage <= 4 ? tunables().kb_per_stage : 2);
+  // k-blocks a stage, except for wide tiles, whose two threads have twice the clocks for the same work, and
+  // beside the gradient's two staging sets
+  const int epi = l.epi == kEpiGatedGrad && t[0].num_kb >= kGradDeepMinKb ? kEpiGatedGradDeep : l.epi;
+  const int want_kb = tunables().kb_per_stage >= 1 && tunables().kb_per_stage <= 4 ? tunables().kb_per_stage : 2;
+  p.kb_per_stage = p.groups == 2 || epi == kEpiGatedGrad ? 1 : want_kb;
   const size_t stage = p.kb_per_stage * (kNarrowABytes + static_cast<size_t>(p.groups) * half_n * 128);
-  const size_t fixed = narrow_fixed_bytes(l.epi);
+  const size_t fixed = narrow_fixed_bytes(epi);
   const int stages = static_cast<int>((kMaxDynSmem - fixed) / stage);
   if (stages < 1) return -1;
   p.num_stages = stages > kNarrowMaxStages ? kNarrowMaxStages : stages;
@@ -457,11 +462,11 @@ int launch_pair(DeviceState* st, const NarrowLaunch& l, const NarrowTask* t, int
   p.status = st->status;
   p.spin_budget = st->spin_budget;
   const int clusters = p.total_units < st->max_clusters ? p.total_units : st->max_clusters;
-  const NarrowKernel<N> k = pair_kernel<N>(l.in.kind, l.epi, l.out_code);
+  const NarrowKernel<N> k = pair_kernel<N>(l.in.kind, epi, l.out_code);
   if (k == nullptr || clusters < 1) return -1;
   // All of the SM's shared memory, whatever the stages need: the kernel takes all of tensor memory, and no
   // CTA that wants columns too may come to wait for them beside it.
-  if (launch_dependent(k, 2 * clusters, l.epi == kEpiGatedGrad ? kNarrowThreads<kEpiGatedGrad> : kNarrowThreads<kEpiStore>, kMaxDynSmem, stream, p) != 0) return -1;
+  if (launch_dependent(k, 2 * clusters, epi_grad(epi) ? kNarrowThreads<kEpiGatedGrad> : kNarrowThreads<kEpiStore>, kMaxDynSmem, stream, p) != 0) return -1;
   t_last = LastCall{12, plan.block_n, t[0].split, 2 * clusters};
 
   NarrowReduceParams r;

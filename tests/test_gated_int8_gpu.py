@@ -123,6 +123,15 @@ def test_backward_matches_64_bits(gpu, rows, d, f, dtype):
         _close(g, w, 1.01 * b + e * w.abs() + floor, name)
 
 
+# deep first products (the gradient's main loop covers its epilogue): odd widths, a K that ends inside a
+# k-block, tiles past the last row and column, several tiles per CTA; same inputs and bounds as above
+@pytest.mark.parametrize("dtype", ["bfloat16", "float16", "float32"])
+@pytest.mark.parametrize("rows,d,f", [(1, 1600, 130), (130, 1537, 517), (257, 1536, 1024), (700, 2056, 4100),
+                                      (2050, 1664, 3001)])
+def test_backward_of_deep_products_matches_64_bits(gpu, rows, d, f, dtype):
+    test_backward_matches_64_bits(gpu, rows, d, f, dtype)
+
+
 def _quant64(x):
     """The definition, in the 32-bit arithmetic it names."""
     import torch
